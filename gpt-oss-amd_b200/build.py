@@ -20,7 +20,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libmoe_b200.so")
 OUT_TEST_AIDS = os.path.join(HERE, "libmoe_b200_testaids.so")
-SOURCES = ["moe_b200.cu"]
+SOURCES = ["moe_b200.cu", "ops.cu"]
 
 
 def _nccl_dirs():
@@ -56,7 +56,7 @@ def _compile(out: str, defines: tuple, verbose: bool) -> None:
     inc, lib = _nccl_dirs()
     cmd = [
         nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
-        "-shared", "-Xcompiler", "-fPIC", "-ccbin", "/usr/bin/g++",
+        "-t", str(len(SOURCES)), "-shared", "-Xcompiler", "-fPIC", "-ccbin", "/usr/bin/g++",
         "-I", inc, "-L", lib, "-l:libnccl.so.2",
         "-Xlinker", f"-rpath={lib}",
         "-o", out,

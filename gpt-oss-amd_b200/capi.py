@@ -13,7 +13,10 @@ LIB_PATH = os.environ.get("MOE_B200_LIB") or os.path.join(_HERE, "libmoe_b200.so
 TEST_AIDS_LIB_PATH = os.path.join(_HERE, "libmoe_b200_testaids.so")
 
 OK, ERR_INVALID, ERR_CUDA, ERR_NO_DEVICE, ERR_NOT_LOADED, ERR_DEVICE, ERR_NCCL, ERR_UNSUPPORTED = range(8)
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_F16, DTYPE_E4M3 = range(4)
+SCALE_NONE, SCALE_ROW, SCALE_G32, SCALE_G64, SCALE_G128, SCALE_MX = range(6)
+SCORE_SOFTMAX, SCORE_SIGMOID = range(2)
+W4_MXFP4, W4_INT4 = range(2)
 GEMM_TCGEN05 = 0
 GEMM_MMA_SYNC = 1  # exists in the test-aids build only
 EP_PEER_EXPORT_BYTES = 256
@@ -31,7 +34,7 @@ SYMBOLS = [
     "moe_b200_ep_peer_resync", "moe_b200_expert_file_info", "moe_b200_load_experts_file",
     "moe_b200_request_queue_create", "moe_b200_request_queue_destroy", "moe_b200_batcher_create",
     "moe_b200_batcher_destroy", "moe_b200_batcher_begin_step", "moe_b200_batcher_end_step",
-    "moe_b200_batcher_stats",
+    "moe_b200_batcher_stats", "moe_b200_add_rmsnorm", "moe_b200_route_logits", "moe_b200_w4_matvec",
 ]
 N_STAGES = 11
 STAGE_NAMES = ["route", "plan", "permute", "dispatch", "regroup", "gemm1", "gemm2", "return",
@@ -46,6 +49,13 @@ class Config(ctypes.Structure):
         ("swiglu_limit", ctypes.c_float), ("max_tokens", ctypes.c_int),
         ("ep_rank", ctypes.c_int), ("ep_size", ctypes.c_int), ("device", ctypes.c_int),
         ("gemm_impl", ctypes.c_int),
+    ]
+
+
+class W4Matrix(ctypes.Structure):
+    _fields_ = [
+        ("format", ctypes.c_int), ("group", ctypes.c_int), ("n_mats", ctypes.c_int), ("rows", ctypes.c_int),
+        ("cols", ctypes.c_int), ("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("bias", ctypes.c_void_p),
     ]
 
 
@@ -90,6 +100,10 @@ def _bind(L: ctypes.CDLL) -> ctypes.CDLL:
     L.moe_b200_ep_peer_enable.argtypes = [vp, ctypes.c_char_p]
     L.moe_b200_ep_peer_sequence.argtypes = [vp]
     L.moe_b200_ep_peer_resync.argtypes = [vp, ci]
+    ll, cf = ctypes.c_longlong, ctypes.c_float
+    L.moe_b200_add_rmsnorm.argtypes = [vp, ci, ll, vp, ci, ll, vp, ll, vp, ci, cf, ci, ci, vp, ci, ll, vp, ll, vp, ci, vp]
+    L.moe_b200_route_logits.argtypes = [vp, ci, ll, ci, ci, ci, ci, vp, ci, ci, ci, ci, cf, vp, vp, vp, vp]
+    L.moe_b200_w4_matvec.argtypes = [ctypes.POINTER(W4Matrix), vp, ci, ll, vp, ci, ci, ci, vp, ci, cf, cf, vp, ci, ll, vp]
     fp = ctypes.POINTER(ctypes.c_float)
     L.moe_b200_expert_file_info.argtypes = [ctypes.c_char_p, ip, ip, ip, ip, ip, fp,
                                             ctypes.POINTER(ctypes.c_ulonglong)]

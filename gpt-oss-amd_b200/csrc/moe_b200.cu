@@ -14,6 +14,7 @@
 #include "batcher.hpp"
 #include "common.cuh"
 #include "ep.cuh"
+#include "error.hpp"
 #include "expert_file.hpp"
 #ifdef MOE_B200_TEST_AIDS
 #include "gemm_mma.cuh"
@@ -27,8 +28,6 @@
 using namespace moe;
 
 namespace {
-
-std::string g_create_error;
 
 struct LayerWeights {
     uint16_t* w_router = nullptr;  // [E, H] bf16
@@ -114,7 +113,7 @@ moe_b200_status fail(moe_b200_handle h, moe_b200_status st, const std::string& m
     if (h)
         h->err = msg;
     else
-        g_create_error = msg;
+        snprintf(moe::thread_error(), moe::THREAD_ERROR_BYTES, "%s", msg.c_str());
     return st;
 }
 
@@ -875,7 +874,7 @@ moe_b200_status moe_b200_create(const moe_b200_config* cfg, moe_b200_handle* out
     auto bail = [&](moe_b200_status s) {
         std::string e = h->err;
         moe_b200_destroy(h);
-        g_create_error = e;
+        fail(nullptr, MOE_B200_ERR_CUDA, e);
         return s;
     };
     if (cudaSetDevice(c.device) != cudaSuccess)
@@ -1396,7 +1395,7 @@ moe_b200_status moe_b200_ep_unique_id(char id_out[128]) {
     std::string err;
     moe_b200_status st = (moe_b200_status)ep::unique_id(id_out, err);
     if (st)
-        g_create_error = err;
+        fail(nullptr, MOE_B200_ERR_NCCL, err);
     return st;
 }
 
@@ -1524,7 +1523,7 @@ void moe_b200_batcher_stats(moe_b200_batcher b, long long* steps, long long* row
 size_t moe_b200_device_bytes(moe_b200_handle h) { return h ? h->device_bytes : 0; }
 
 const char* moe_b200_last_error(moe_b200_handle h) {
-    return h ? h->err.c_str() : g_create_error.c_str();
+    return h ? h->err.c_str() : moe::thread_error();
 }
 
 moe_b200_status moe_b200_device_status(moe_b200_handle h, int* status_word) {

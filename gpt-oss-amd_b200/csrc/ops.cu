@@ -1,0 +1,282 @@
+// Host side of the stand-alone operators of include/moe_b200.h: argument checks and launches.
+// They need no handle, allocate nothing and keep nothing between calls.
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <cstdarg>
+#include <cstdio>
+
+#include "error.hpp"
+#include "op_matvec.cuh"
+#include "op_norm.cuh"
+#include "op_route.cuh"
+
+using namespace moe::op;
+
+namespace {
+
+constexpr int MAX_DEVICES = 64;
+
+moe_b200_status refuse(moe_b200_status st, const char* fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(moe::thread_error(), moe::THREAD_ERROR_BYTES, fmt, ap);
+    va_end(ap);
+    return st;
+}
+
+#define INVALID(...) return refuse(MOE_B200_ERR_INVALID, __VA_ARGS__)
+
+// Device and SM count of the calling thread's current device.
+moe_b200_status current_device(int* dev, int* sms) {
+    static std::atomic<int> cache[MAX_DEVICES];
+    if (cudaGetDevice(dev) != cudaSuccess) {
+        cudaGetLastError();
+        return refuse(MOE_B200_ERR_NO_DEVICE, "no CUDA device; this library has no CPU path");
+    }
+    int n = *dev < MAX_DEVICES ? cache[*dev].load(std::memory_order_relaxed) : 0;
+    if (n == 0) {
+        cudaError_t e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, *dev);
+        if (e != cudaSuccess)
+            return refuse(MOE_B200_ERR_CUDA, "cudaDeviceGetAttribute: %s", cudaGetErrorString(e));
+        if (*dev < MAX_DEVICES)
+            cache[*dev].store(n, std::memory_order_relaxed);
+    }
+    *sms = n;
+    return MOE_B200_OK;
+}
+
+moe_b200_status launched(const char* what, cudaError_t e) {
+    return e == cudaSuccess ? MOE_B200_OK : refuse(MOE_B200_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
+bool is_float_type(int dtype) {
+    return dtype == MOE_B200_DTYPE_F32 || dtype == MOE_B200_DTYPE_BF16 || dtype == MOE_B200_DTYPE_F16;
+}
+
+bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// Rows of `stride` elements of `size` bytes on `n`-byte boundaries.
+bool rows_aligned(const void* p, long long stride, int size, size_t n) {
+    return aligned(p, n) && ((unsigned long long)stride * (unsigned)size) % n == 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+moe_b200_status moe_b200_add_rmsnorm(const void* x, int x_dtype, long long x_stride, const void* residual,
+                                     int residual_dtype, long long residual_stride, void* residual_out,
+                                     long long residual_out_stride, const void* weight, int weight_dtype, float eps,
+                                     int n_rows, int hidden_dim, void* y, int y_dtype, long long y_stride, void* q,
+                                     long long q_stride, void* q_scales, int q_kind, moe_b200_stream stream) {
+    const int H = hidden_dim;
+    if (n_rows < 0 || H <= 0 || H > MOE_B200_ADD_RMSNORM_MAX_HIDDEN)
+        INVALID("moe_b200_add_rmsnorm: needs n_rows >= 0 and hidden_dim in 1..%d", MOE_B200_ADD_RMSNORM_MAX_HIDDEN);
+    if (!is_float_type(x_dtype) || !is_float_type(weight_dtype) || (residual && !is_float_type(residual_dtype)) ||
+        (y && !is_float_type(y_dtype)))
+        INVALID("moe_b200_add_rmsnorm: x, residual, weight and y are f32, bf16 or f16");
+    if (!(eps >= 0.f) || eps > 3.0e38f)
+        INVALID("moe_b200_add_rmsnorm: eps must be finite and not negative");
+    int group = 0, mx = 0, n_scales = 1;
+    if (q) {
+        switch (q_kind) {
+            case MOE_B200_SCALE_ROW: break;
+            case MOE_B200_SCALE_G32: group = 32; break;
+            case MOE_B200_SCALE_G64: group = 64; break;
+            case MOE_B200_SCALE_G128: group = 128; break;
+            case MOE_B200_SCALE_MX: group = 32, mx = 1; break;
+            default: INVALID("moe_b200_add_rmsnorm: unknown scale kind %d", q_kind);
+        }
+        n_scales = group ? (H + group - 1) / group : 1;
+    }
+    if (n_rows == 0)
+        return MOE_B200_OK;
+    if (!y && !q)
+        INVALID("moe_b200_add_rmsnorm: neither y nor q asked for");
+    if (residual_out && !residual)
+        INVALID("moe_b200_add_rmsnorm: residual_out without residual");
+    if (!x || !weight || (q && !q_scales))
+        INVALID("moe_b200_add_rmsnorm: null pointer");
+    if (x_stride < 0 || (residual && residual_stride < 0) || (residual_out && n_rows > 1 && residual_out_stride < H) ||
+        (y && n_rows > 1 && y_stride < H) || (q && n_rows > 1 && q_stride < H))
+        INVALID("moe_b200_add_rmsnorm: strides of inputs are not negative, rows of outputs do not overlap");
+    if (!aligned(x, size_of(x_dtype)) || !aligned(weight, size_of(weight_dtype)) ||
+        (residual && !aligned(residual, size_of(residual_dtype))) ||
+        (residual_out && !aligned(residual_out, size_of(residual_dtype))) || (y && !aligned(y, size_of(y_dtype))) ||
+        (q && !mx && !aligned(q_scales, 4)))
+        INVALID("moe_b200_add_rmsnorm: a pointer is not on a boundary of its element type");
+    int dev, sms;
+    if (moe_b200_status st = current_device(&dev, &sms))
+        return st;
+    NormArgs a{x, x_stride, x_dtype, residual, residual_out, residual_stride, residual_out_stride, residual_dtype,
+               weight, weight_dtype, eps, H, y, y_stride, y_dtype, static_cast<uint8_t*>(q), q_stride, q_scales,
+               n_scales, group, mx};
+    const bool vec = H % 8 == 0 && rows_aligned(x, x_stride, size_of(x_dtype), 16) && aligned(weight, 16) &&
+                     (!residual || rows_aligned(residual, residual_stride, size_of(residual_dtype), 16)) &&
+                     (!residual_out || rows_aligned(residual_out, residual_out_stride, size_of(residual_dtype), 16)) &&
+                     (!y || rows_aligned(y, y_stride, size_of(y_dtype), 16)) && (!q || rows_aligned(q, q_stride, 1, 8));
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const int chunks = (H + 255) / 256;  // of a warp
+    const int nv = chunks <= 32 ? (n_rows > 2 * sms && chunks > 4 ? 2 : 1) : chunks <= 64 ? 2 : 4;
+    const int threads = 32 * ((chunks + nv - 1) / nv);
+    auto kernel = vec ? (nv == 1 ? add_rmsnorm_kernel<true, 1> : nv == 2 ? add_rmsnorm_kernel<true, 2> : add_rmsnorm_kernel<true, 4>)
+                      : (nv == 1 ? add_rmsnorm_kernel<false, 1> : nv == 2 ? add_rmsnorm_kernel<false, 2> : add_rmsnorm_kernel<false, 4>);
+    kernel<<<n_rows, threads, 0, st>>>(a);
+    return launched("moe_b200_add_rmsnorm", cudaGetLastError());
+}
+
+moe_b200_status moe_b200_route_logits(const void* logits, int dtype, long long stride, int n_tokens, int n_experts,
+                                      int experts_per_token, int score, const float* bias, int n_groups,
+                                      int topk_groups, int group_top, int renormalize, float scale, int* topk_i,
+                                      float* topk_w, int* expert_counts, moe_b200_stream stream) {
+    const int E = n_experts, K = experts_per_token;
+    if (n_tokens < 0 || E <= 0 || E > MOE_B200_ROUTE_LOGITS_MAX_EXPERTS)
+        INVALID("moe_b200_route_logits: needs n_tokens >= 0 and n_experts in 1..%d", MOE_B200_ROUTE_LOGITS_MAX_EXPERTS);
+    if (K <= 0 || K > MOE_B200_ROUTE_LOGITS_MAX_K || K > E)
+        INVALID("moe_b200_route_logits: experts_per_token must be in 1..min(%d, n_experts)", MOE_B200_ROUTE_LOGITS_MAX_K);
+    if (!is_float_type(dtype))
+        INVALID("moe_b200_route_logits: logits are f32, bf16 or f16");
+    if (score != MOE_B200_SCORE_SOFTMAX && score != MOE_B200_SCORE_SIGMOID)
+        INVALID("moe_b200_route_logits: unknown score %d", score);
+    if (n_groups < 1 || n_groups > ROUTE_MAX_GROUPS || E % n_groups || topk_groups < 1 || topk_groups > n_groups)
+        INVALID("moe_b200_route_logits: n_groups must be in 1..%d and divide n_experts, topk_groups in 1..n_groups",
+                ROUTE_MAX_GROUPS);
+    if (n_groups > 1 && (group_top < 1 || group_top > 2 || group_top > E / n_groups))
+        INVALID("moe_b200_route_logits: a group is scored by its best or its two best experts");
+    if ((long long)topk_groups * (E / n_groups) < K)
+        INVALID("moe_b200_route_logits: the groups kept hold fewer than experts_per_token experts");
+    if (!(scale > -3.0e38f && scale < 3.0e38f))
+        INVALID("moe_b200_route_logits: scale must be finite");
+    if (n_tokens > 0 && (!logits || !topk_i || !topk_w))
+        INVALID("moe_b200_route_logits: null pointer");
+    if (stride < 0)
+        INVALID("moe_b200_route_logits: negative stride");
+    if (!aligned(logits, size_of(dtype)) || !aligned(bias, 4) || !aligned(topk_i, 4) || !aligned(topk_w, 4) ||
+        !aligned(expert_counts, 4))
+        INVALID("moe_b200_route_logits: a pointer is not on a boundary of its element type");
+    if (n_tokens == 0 && !expert_counts)
+        return MOE_B200_OK;
+    int dev, sms;
+    if (moe_b200_status st = current_device(&dev, &sms))
+        return st;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (expert_counts) {
+        cudaError_t e = cudaMemsetAsync(expert_counts, 0, sizeof(int) * (size_t)E, st);
+        if (e != cudaSuccess)
+            return launched("moe_b200_route_logits: counts", e);
+        if (n_tokens == 0)
+            return MOE_B200_OK;
+    }
+    LogitsArgs a{logits, stride, dtype, n_tokens, E, K, score == MOE_B200_SCORE_SIGMOID, bias, n_groups, topk_groups,
+                 group_top, renormalize != 0, scale, topk_i, topk_w, expert_counts};
+    const int warps = n_tokens >= ROUTE_WARPS * sms ? ROUTE_WARPS : 1;
+    const int want = (n_tokens + warps - 1) / warps, most = 32 * sms;
+    const int grid = want < most ? want : most;
+    auto kernel = E <= 32 ? route_logits_kernel<1> : E <= 64 ? route_logits_kernel<2> : E <= 128 ? route_logits_kernel<4>
+                  : E <= 256 ? route_logits_kernel<8> : route_logits_kernel<16>;
+    kernel<<<grid, 32 * warps, 0, st>>>(a);
+    return launched("moe_b200_route_logits", cudaGetLastError());
+}
+
+moe_b200_status moe_b200_w4_matvec(const moe_b200_w4_matrix* w, const void* x, int x_dtype, long long x_stride,
+                                   const void* x_scales, int x_scale_kind, int n_rows, int rows_per_x, const int* ids,
+                                   int swiglu, float swiglu_alpha, float swiglu_limit, void* out, int out_dtype,
+                                   long long out_stride, moe_b200_stream stream) {
+    if (!w)
+        INVALID("moe_b200_w4_matvec: null pointer");
+    const bool int4 = w->format == MOE_B200_W4_INT4;
+    if (!int4 && w->format != MOE_B200_W4_MXFP4)
+        INVALID("moe_b200_w4_matvec: unknown weight format %d", w->format);
+    if (int4 ? (w->group != 32 && w->group != 64 && w->group != 128) : w->group != 32)
+        INVALID("moe_b200_w4_matvec: groups of 32 (mxfp4), or 32, 64 or 128 (int4) columns");
+    const int N = w->rows, K = w->cols;
+    if (N <= 0 || N > MOE_B200_W4_MATVEC_MAX_OUT || K <= 0 || K > MOE_B200_W4_MATVEC_MAX_IN || K % w->group || w->n_mats <= 0)
+        INVALID("moe_b200_w4_matvec: needs rows in 1..%d, cols a multiple of the group up to %d, n_mats >= 1",
+                MOE_B200_W4_MATVEC_MAX_OUT, MOE_B200_W4_MATVEC_MAX_IN);
+    if (n_rows < 0 || n_rows > MOE_B200_W4_MATVEC_MAX_ROWS || rows_per_x <= 0)
+        INVALID("moe_b200_w4_matvec: n_rows must be in 0..%d (larger batches are matrix products), rows_per_x >= 1",
+                MOE_B200_W4_MATVEC_MAX_ROWS);
+    if (!ids && w->n_mats != 1)
+        INVALID("moe_b200_w4_matvec: several matrices need ids");
+    if (x_dtype != MOE_B200_DTYPE_BF16 && x_dtype != MOE_B200_DTYPE_F16 && x_dtype != MOE_B200_DTYPE_E4M3)
+        INVALID("moe_b200_w4_matvec: x is bf16, f16 or e4m3");
+    if ((x_dtype == MOE_B200_DTYPE_E4M3) != (x_scale_kind != MOE_B200_SCALE_NONE))
+        INVALID("moe_b200_w4_matvec: e4m3 rows need scales, bf16 and f16 rows have none");
+    if (!is_float_type(out_dtype))
+        INVALID("moe_b200_w4_matvec: out is f32, bf16 or f16");
+    if (swiglu && (N % 2 || !(swiglu_limit >= 0.f) || swiglu_alpha != swiglu_alpha))
+        INVALID("moe_b200_w4_matvec: SwiGLU needs an even number of rows (gate, up) and a limit");
+    int n_xs = 0, xs_shift = 31;
+    switch (x_scale_kind) {
+        case MOE_B200_SCALE_NONE: break;
+        case MOE_B200_SCALE_ROW: n_xs = 1; break;
+        case MOE_B200_SCALE_MX:
+        case MOE_B200_SCALE_G32: xs_shift = 0; break;
+        case MOE_B200_SCALE_G64: xs_shift = 1; break;
+        case MOE_B200_SCALE_G128: xs_shift = 2; break;
+        default: INVALID("moe_b200_w4_matvec: unknown scale kind %d", x_scale_kind);
+    }
+    if (xs_shift != 31)
+        n_xs = (K + (32 << xs_shift) - 1) / (32 << xs_shift);
+    if (n_rows == 0)
+        return MOE_B200_OK;
+    if (!w->codes || !w->scales || !x || !out || (x_scale_kind != MOE_B200_SCALE_NONE && !x_scales))
+        INVALID("moe_b200_w4_matvec: null pointer");
+    const int n_out = swiglu ? N / 2 : N;
+    if (x_stride < 0 || (n_rows > 1 && out_stride < n_out))
+        INVALID("moe_b200_w4_matvec: x_stride is not negative, rows of out do not overlap");
+    if (!aligned(w->codes, 16) || !rows_aligned(x, x_stride, size_of(x_dtype), x_dtype == MOE_B200_DTYPE_E4M3 ? 8 : 16))
+        INVALID("moe_b200_w4_matvec: codes and rows of x must be 16-byte aligned (rows of e4m3 8-byte aligned)");
+    if ((int4 && !aligned(w->scales, 2)) || !aligned(w->bias, 4) || !aligned(ids, 4) || !aligned(out, size_of(out_dtype)) ||
+        (n_xs && x_scale_kind != MOE_B200_SCALE_MX && !aligned(x_scales, 4)))
+        INVALID("moe_b200_w4_matvec: a pointer is not on a boundary of its element type");
+    int dev, sms;
+    if (moe_b200_status st = current_device(&dev, &sms))
+        return st;
+    MatvecArgs a{};
+    a.codes = w->codes;
+    a.scales = w->scales;
+    a.bias = w->bias;
+    a.n_mats = w->n_mats;
+    a.N = N;
+    a.K = K;
+    a.group_shift = w->group == 128 ? 2 : w->group == 64 ? 1 : 0;
+    a.x = x;
+    a.x_stride = x_stride;
+    a.x_dtype = x_dtype;
+    a.x_scales = n_xs ? x_scales : nullptr;
+    a.n_xs = n_xs;
+    a.xs_shift = xs_shift;
+    a.xs_mx = x_scale_kind == MOE_B200_SCALE_MX;
+    a.R = n_rows;
+    a.rows_per_x = rows_per_x;
+    a.ids = ids;
+    a.swiglu = swiglu != 0;
+    a.alpha = swiglu_alpha;
+    a.limit = swiglu_limit;
+    a.out = out;
+    a.out_stride = out_stride;
+    a.out_dtype = out_dtype;
+    a.n_tiles = (N + MV_TILE - 1) / MV_TILE;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+
+    // rows of x per pass over the weights: 2, 4 or 8, as many as there are and shared memory holds
+    int pairs = n_rows <= 2 ? 1 : n_rows <= 4 ? 2 : 4;
+    while (pairs > 1 && mv_smem_bytes(K, 2 * pairs) > 200 * 1024)
+        pairs /= 2;
+    const size_t smem = mv_smem_bytes(K, 2 * pairs);
+    auto kernel = int4 ? (pairs == 1 ? w4_matvec_kernel<true, 1> : pairs == 2 ? w4_matvec_kernel<true, 2> : w4_matvec_kernel<true, 4>)
+                       : (pairs == 1 ? w4_matvec_kernel<false, 1> : pairs == 2 ? w4_matvec_kernel<false, 2> : w4_matvec_kernel<false, 4>);
+    if (smem > 32 * 1024) {  // with the fixed part more than a block has without asking
+        cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+        if (e != cudaSuccess)
+            return launched("moe_b200_w4_matvec: shared memory", e);
+    }
+    const long long passes = ids ? n_rows : (n_rows + 2 * pairs - 1) / (2 * pairs);
+    const long long items = passes * a.n_tiles, most = (smem > 90 * 1024 ? 1 : 2) * (long long)sms;
+    kernel<<<(unsigned)(items < most ? items : most), MV_THREADS, smem, st>>>(a);
+    return launched("moe_b200_w4_matvec", cudaGetLastError());
+}
+
+}  // extern "C"

@@ -49,9 +49,12 @@ typedef enum {
     MOE_B200_ERR_UNSUPPORTED = 7  /* valid input outside what is implemented  */
 } moe_b200_status;
 
-/* Activation element types accepted by moe_b200_forward(). */
+/* Activation element types.  moe_b200_forward() takes the first two; the stand-alone
+ * operators at the end of this file say which they take. */
 #define MOE_B200_DTYPE_F32 0  /* the engine's s->t buffer (include/model.hpp:113) */
 #define MOE_B200_DTYPE_BF16 1 /* already-rounded activations                      */
+#define MOE_B200_DTYPE_F16 2
+#define MOE_B200_DTYPE_E4M3 3 /* 8 bits: 4 of exponent, 3 of mantissa, largest 448 */
 
 /* The expert GEMMs are tcgen05 kernels (CTA pairs for large batches, token rows
  * on the accumulator lanes for small ones); moe_b200_config.gemm_impl must be
@@ -272,8 +275,9 @@ void moe_b200_batcher_stats(moe_b200_batcher b, long long* steps, long long* row
 
 /* Bytes of device memory the handle holds (weights + workspace). */
 size_t moe_b200_device_bytes(moe_b200_handle h);
-/* Text of the last error on this handle (or of the last failed create when h
- * is NULL).  Never NULL. */
+/* Text of the last error on this handle or, when h is NULL, of the calling
+ * thread's last failed call that has no handle (create and the stand-alone
+ * functions).  Never NULL. */
 const char* moe_b200_last_error(moe_b200_handle h);
 /* Reads AND CLEARS the device status word (synchronises the device): 0 = no
  * kernel has reported a problem since the last read; otherwise the code of the
@@ -382,6 +386,114 @@ moe_b200_status moe_b200_route_noalloc(const void* t, int t_dtype, int n_tokens,
                                        int n_experts, int experts_per_token, int* topk_i_out,
                                        float* topk_w_out, int* expert_counts_out,
                                        int* expert_offsets_out, moe_b200_stream stream);
+
+/* Stand-alone operators: the steps around and beside the MoE block for tensors of
+ * the caller's own.  (The reference has them inside its engine only: rmsnorm and
+ * the residual add src/run.cpp:306-319,709-711, router selection src/run.cpp:
+ * 373-404, matrix-vector products src/run.cpp:341-354.)  No handle, no
+ * allocation, nothing kept between calls: calls may overlap on any streams and
+ * host threads and may be captured into graphs.  Device pointers and a stream of
+ * the current device.  Strides are in elements between two rows.  Nothing outside
+ * the stated rows and columns is written. */
+
+/* Scales of 8-bit rows: none, one fp32 per row, one fp32 per group of 32 / 64 /
+ * 128 neighbouring columns (the last group may be shorter), one e8m0 byte per
+ * group of 32 (MX).  Layout [rows, scales per row], no gaps. */
+#define MOE_B200_SCALE_NONE 0
+#define MOE_B200_SCALE_ROW 1
+#define MOE_B200_SCALE_G32 2
+#define MOE_B200_SCALE_G64 3
+#define MOE_B200_SCALE_G128 4
+#define MOE_B200_SCALE_MX 5
+
+/* Residual add, RMSNorm and 8-bit output in one pass:
+ *   r = x + residual (x alone when residual is NULL)
+ *   residual_out = r                                        optional
+ *   y = r / sqrt(mean(r^2) + eps) * weight                  optional
+ *   q = e4m3(y / scale), q_scales = scale                   optional
+ * x [n_rows, H], residual, y f32, bf16 or f16; weight [H] of any of the three;
+ * residual_out has residual's type.  All in fp32, each output rounded once; the
+ * norm is of r before it is rounded to residual_out's type.  residual_out may be
+ * residual itself; any output may be an input of the same type and stride; other
+ * overlaps are the caller's error.
+ * A group's fp32 scale is its largest |y| / 448 (1 where that is 0, and not
+ * below 2^-126); an MX scale is the least power of two s with largest |y| <= 448 s
+ * (2^0 where that is 0, not below 2^-127).  Largest means of the numbers: NaN is
+ * passed over there and becomes a NaN code.  Any H up to
+ * MOE_B200_ADD_RMSNORM_MAX_HIDDEN, any stride; rows on 16-byte boundaries with H a
+ * multiple of 8 take the fast path. */
+#define MOE_B200_ADD_RMSNORM_MAX_HIDDEN 32768
+moe_b200_status moe_b200_add_rmsnorm(const void* x, int x_dtype, long long x_stride, const void* residual,
+                                     int residual_dtype, long long residual_stride, void* residual_out,
+                                     long long residual_out_stride, const void* weight, int weight_dtype, float eps,
+                                     int n_rows, int hidden_dim, void* y, int y_dtype, long long y_stride, void* q,
+                                     long long q_stride, void* q_scales, int q_kind, moe_b200_stream stream);
+
+/* Experts and weights from router logits [n_tokens, n_experts] (f32, bf16, f16):
+ *   p_e   = softmax over the experts, or the sigmoid, of the logits
+ *   key_e = p_e + bias_e with a bias (f32 [n_experts], for balance: it moves the
+ *           choice, not the weights); without one the order of the logits
+ *   groups: with n_groups > 1 the experts form n_groups equal neighbouring groups,
+ *           scored by the sum of their group_top (1 or 2) largest keys (of p_e
+ *           where there is no bias); experts of the topk_groups best take part
+ *   topk_i = the K experts of the largest keys in falling order, ties (of experts
+ *           and of groups) to the lower index
+ *   topk_w = p of the selected, divided by their sum when renormalize != 0, times
+ *           scale.  softmax with renormalize is the softmax over the selected.
+ * The order is that of keys computed in 64 bits.  An expert whose logit (or bias)
+ * is -inf or NaN takes no part: softmax and groups do not count it, and a slot for
+ * which no expert is left gets index -1 and weight 0.  +inf counts as the largest
+ * finite value.  expert_counts (optional, [n_experts]): slots that went to each
+ * expert, overwritten. */
+#define MOE_B200_SCORE_SOFTMAX 0
+#define MOE_B200_SCORE_SIGMOID 1
+#define MOE_B200_ROUTE_LOGITS_MAX_EXPERTS 512
+#define MOE_B200_ROUTE_LOGITS_MAX_K 16
+moe_b200_status moe_b200_route_logits(const void* logits, int dtype, long long stride, int n_tokens, int n_experts,
+                                      int experts_per_token, int score, const float* bias, int n_groups,
+                                      int topk_groups, int group_top, int renormalize, float scale, int* topk_i,
+                                      float* topk_w, int* expert_counts, moe_b200_stream stream);
+
+/* A stack of matrices in 4 bits.  Two codes per byte, the even column in the low
+ * half; codes 16-byte aligned.
+ *   MXFP4  e2m1 codes, scales e8m0 bytes per group of 32 (checkpoint layout: the
+ *          blocks and scales of moe_b200_set_experts_mxfp4), value 2^(byte - 127)
+ *          for every byte
+ *   INT4   value code - 8, scales bf16 per group of 32, 64 or 128 */
+#define MOE_B200_W4_MXFP4 0
+#define MOE_B200_W4_INT4 1
+typedef struct {
+    int format;
+    int group;             /* columns per scale                            */
+    int n_mats;            /* matrices, one behind the other               */
+    int rows;              /* outputs of one matrix                        */
+    int cols;              /* inputs, a multiple of the group              */
+    const uint8_t* codes;  /* [n_mats, rows, cols / 2]                     */
+    const void* scales;    /* [n_mats, rows, cols / group]                 */
+    const float* bias;     /* [n_mats, rows] or NULL                       */
+} moe_b200_w4_matrix;
+
+/* Products of a few rows with 4-bit matrices:
+ *   out[m] = W[ids[m]] x[m / rows_per_x] + bias[ids[m]]     (ids NULL: the one matrix)
+ * With the indices of a routing call and rows_per_x = K these are the experts'
+ * products of n_rows / K tokens; a matrix that several rows ask for is read once
+ * per 8 of them (4 or 2 for very long rows).  A row whose id is not in 0..n_mats-1
+ * (-1 of an empty slot) becomes zeros.
+ *   x      [rows, cols] bf16 or f16, or e4m3 with x_scales of kind x_scale_kind (as
+ *          moe_b200_add_rmsnorm writes them).  x_stride may be 0
+ *   swiglu != 0: rows 2i are gates, 2i + 1 ups, and out[m, i] is the clamped
+ *          SwiGLU of moe_b200_config (alpha, limit): g = min(gate, limit),
+ *          u = clamp(up, +-limit), g sigmoid(alpha g) (u + 1)
+ *   out    [n_rows, rows] (rows / 2 with swiglu) f32, bf16 or f16
+ * Products are exact and summed in fp32; one rounding at the end.  Row addresses
+ * of x must be 16-byte aligned (8 bytes for e4m3). */
+#define MOE_B200_W4_MATVEC_MAX_ROWS 256
+#define MOE_B200_W4_MATVEC_MAX_IN 32768
+#define MOE_B200_W4_MATVEC_MAX_OUT 4194304
+moe_b200_status moe_b200_w4_matvec(const moe_b200_w4_matrix* w, const void* x, int x_dtype, long long x_stride,
+                                   const void* x_scales, int x_scale_kind, int n_rows, int rows_per_x, const int* ids,
+                                   int swiglu, float swiglu_alpha, float swiglu_limit, void* out, int out_dtype,
+                                   long long out_stride, moe_b200_stream stream);
 
 /* Library build info, e.g. "moe_b200 0.1 sm_100a". */
 const char* moe_b200_version(void);
