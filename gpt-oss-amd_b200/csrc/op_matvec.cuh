@@ -34,7 +34,12 @@ constexpr int MV_WARPS = 8;
 constexpr int MV_THREADS = 32 * MV_WARPS;
 constexpr int MV_TILE = 16;                                   // rows of W per item
 constexpr int MV_MAX_ROWS = MOE_B200_W4_MATVEC_MAX_ROWS;      // one thread per row builds the item list
-constexpr int MV_UB = 3;                                      // steps (128 columns) in flight per warp
+// Ring stages of a warp (two steps of 128 columns each) and blocks per SM with P pairs of x rows: as much in
+// flight as shared memory and registers hold.
+__host__ __device__ constexpr int mv_depth(int P) { return P == 4 ? 2 : 3; }
+constexpr int MV_BLOCKS = 2;
+constexpr int MV_STAGE_BYTES = 2 * 1024 + 256;                // per step: codes of rows 0..7, of rows 8..15; scale words
+constexpr int MV_DIRECT = 3;                                  // SH: scales are loaded where they are used
 static_assert(MV_MAX_ROWS <= MV_THREADS, "one thread per row");
 
 struct MatvecArgs {
@@ -58,12 +63,14 @@ struct MatvecArgs {
     long long out_stride;
     int out_dtype;
     int n_tiles;
+    int ksplit;             // warps that share a tile: 1, 2, 4 or 8, at most the stages of a row
 };
 
-// Shared memory behind the fixed part: x rows in fp16, then their scales per group of 32.
+// Dynamic shared memory: zeros, the rings of the warps, x rows in fp16, then their scales per group of 32.
+__host__ __device__ constexpr int mv_x_at(int P) { return 64 + MV_WARPS * mv_depth(P) * MV_STAGE_BYTES; }
 __host__ __device__ constexpr int mv_steps(int K) { return (K + 127) / 128; }
-__host__ __device__ constexpr size_t mv_smem_bytes(int K, int rows) {
-    return (size_t)rows * mv_steps(K) * (128 * 2 + 4 * 4);
+__host__ __device__ constexpr size_t mv_smem_bytes(int K, int P, int rows) {
+    return mv_x_at(P) + (size_t)rows * mv_steps(K) * (128 * 2 + 4 * 4);
 }
 
 template <bool INT4>
@@ -92,68 +99,103 @@ __device__ __forceinline__ void mv_decode(uint32_t w, uint32_t (&o)[4]) {
     }
 }
 
+// c = a b, and c += a b.
+__device__ __forceinline__ void mv_mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void mv_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// A weight scale as fp32.  An e8m0 byte means 2^(byte - 127) for EVERY byte, 255 included, as in
-// moe_b200_mxfp4_unpack; 2^128 is no fp32 number, so the sums are kept in units of 2: this is
-// 2^(byte - 128), bytes 0 and 1 being subnormals, and the epilogue doubles.
+// Two weight scales as fp32, from the low 16 bits (mxfp4: two bytes) or the 32 bits (int4) of `raw`.
 template <bool INT4>
-__device__ __forceinline__ float mv_scale(uint32_t raw) {
-    if (INT4)
-        return __uint_as_float(raw << 16);
-    return __uint_as_float(raw > 1u ? (raw - 1u) << 23 : 0x00200000u << raw);
+__device__ __forceinline__ float2 mv_scales(uint32_t raw) {
+    if (!INT4)  // e8m0 -> bf16: 2^(byte - 127), byte 0 a subnormal, byte 255 NaN
+        asm("cvt.rn.bf16x2.ue8m0x2 %0, %1;" : "=r"(raw) : "h"((uint16_t)raw));
+    return make_float2(__uint_as_float(raw << 16), __uint_as_float(raw & 0xFFFF0000u));
 }
 
-struct MvStep {  // one step of a lane as loaded: codes of rows g and g + 8, two scales of each
-    uint4 lo, hi;
-    uint32_t s_lo, s_hi;
-};
-
-// The raw scales of groups sg and sg + 1 of a row whose scales start at element `row` (32-column
-// groups past G: 0); mxfp4: bytes 0 and 1 of the result, int4: its halves.
+// The raw scales of groups sg and sg + 1 (sg even) of a row, zeros past the row's G groups; mxfp4: bytes 0 and
+// 1 of the result, int4: its halves.
 template <bool INT4>
-__device__ __forceinline__ uint32_t mv_load_scales(const void* scales, long long row, int sg, int G, int shift, bool paired) {
+__device__ __forceinline__ uint32_t mv_load_scales(const uint8_t* row, int sg, int G, int shift) {
+    uint32_t r = 0;
     if (INT4) {
-        const uint16_t* p = static_cast<const uint16_t*>(scales) + row;
-        if (paired)  // two neighbours on a word boundary
-            return *reinterpret_cast<const uint32_t*>(p + sg);
-        uint32_t r = p[sg >> shift];
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
+        if (sg < G)
+            r = p[sg >> shift];
         if (sg + 1 < G)
             r |= (uint32_t)p[(sg + 1) >> shift] << 16;
-        return r;
+    } else {
+        if (sg < G)
+            r = row[sg];
+        if (sg + 1 < G)
+            r |= (uint32_t)row[sg + 1] << 8;
     }
-    const uint8_t* p = static_cast<const uint8_t*>(scales) + row;
-    if (paired)
-        return *reinterpret_cast<const uint16_t*>(p + sg);
-    uint32_t r = p[sg];
-    if (sg + 1 < G)
-        r |= (uint32_t)p[sg + 1] << 8;
     return r;
 }
 
+// The same from the words of a stage.  A stage's scales start at byte `o` of a row's four words; mv_pick is
+// the byte selector of a lane for its first step, mv_from_words applies it for step h.
+template <bool INT4, int SH>
+__device__ __forceinline__ uint32_t mv_pick(const uint8_t* at, int t) {
+    const uint32_t o = (uint32_t)(reinterpret_cast<uintptr_t>(at) & 3), k = t & 1;
+    if (!INT4)
+        return (o + 2 * k) * 0x11u + 0x7710u;  // bytes 2 and 3 of the result are not used
+    if (SH == 0)
+        return k ? 0x7654u : 0x3210u;
+    return (SH == 1 ? o + 2 * k : o) * 0x1111u + 0x1010u;
+}
+template <bool INT4, int SH>
+__device__ __forceinline__ uint32_t mv_from_words(const uint4& w, uint32_t pick, int h) {
+    if (INT4 && SH == 0)
+        return h ? __byte_perm(w.z, w.w, pick) : __byte_perm(w.x, w.y, pick);
+    if (INT4 && SH == 2)
+        return __byte_perm(w.x, w.y, pick + 0x2222u * h);
+    return h ? __byte_perm(w.y, w.z, pick) : __byte_perm(w.x, w.y, pick);
+}
+
+__device__ __forceinline__ void mv_copy16(int at, const void* src) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(at), "l"(src) : "memory");
+}
+__device__ __forceinline__ void mv_copy4(int at, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at), "l"(src) : "memory");
+}
+__device__ __forceinline__ void mv_copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void mv_copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // P pairs of x rows (columns of the MMA) per pass over the weights.
-template <bool INT4, int P>
-__global__ void __launch_bounds__(MV_THREADS, 2) w4_matvec_kernel(const MatvecArgs a) {
-    constexpr int RP = 2 * P;
+// SH: log2 of 32-column groups per scale, the scales coming through the ring in aligned words; MV_DIRECT where they
+// cannot (an odd number of bf16 scales per row, or scales off a word boundary).
+template <bool INT4, int SH, int P>
+__global__ void __launch_bounds__(MV_THREADS, MV_BLOCKS) w4_matvec_kernel(const MatvecArgs a) {
+    constexpr int RP = 2 * P, DEPTH = mv_depth(P);
     extern __shared__ __align__(16) uint8_t dyn[];
     __shared__ int s_ids[MV_MAX_ROWS];
     __shared__ int s_lead[MV_MAX_ROWS];
     __shared__ int s_rank[MV_MAX_ROWS];
     __shared__ int s_warp_cnt[MV_WARPS];
     __shared__ int s_rows[RP];
-    __shared__ float s_red[2][MV_WARPS][MV_TILE][RP];
+    __shared__ float2 s_red[2][MV_WARPS][P][16];
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int steps = mv_steps(a.K), G = a.K >> 5, SG = G >> a.group_shift;
-    uint16_t* xs = reinterpret_cast<uint16_t*>(dyn);                                     // [RP][steps * 128] fp16
-    float* xsc = reinterpret_cast<float*>(dyn + (size_t)RP * steps * 128 * 2);           // [RP][steps * 4]
+    const int xs_at = mv_x_at(P), xsc_at = xs_at + min(RP, a.R) * steps * 256;
+    uint4* xs = reinterpret_cast<uint4*>(dyn + xs_at);
+    float* xsc = reinterpret_cast<float*>(dyn + xsc_at);
+    if (tid < 4)
+        reinterpret_cast<uint4*>(dyn)[tid] = make_uint4(0, 0, 0, 0);
 
     // the list of leaders: rows that open a pass over their matrix
     int n_lead;
@@ -192,73 +234,102 @@ __global__ void __launch_bounds__(MV_THREADS, 2) w4_matvec_kernel(const MatvecAr
 
     const long long total = (long long)n_lead * a.n_tiles;  // fits an int (checked by the host)
     const int i0 = (int)(total * blockIdx.x / gridDim.x), i1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
-    const int per_warp = (steps + MV_WARPS - 1) / MV_WARPS;
-    const int b0 = min(warp * per_warp, steps), b1 = min(b0 + per_warp, steps);
-    const int units = (per_warp + MV_UB - 1) / MV_UB;  // the same for all warps
-    // two scales with one load: neighbours in memory, on a boundary of their size together
-    const bool paired = a.group_shift == 0 && (G & 1) == 0 &&
-                        (reinterpret_cast<uintptr_t>(a.scales) & (INT4 ? 3u : 1u)) == 0;
+    const int KS = a.ksplit, ks = warp & (KS - 1), slot = warp / KS, n_slots = MV_WARPS / KS;
+    const int half = (steps + 1) >> 1;  // stages of a row
+    const int b0 = 2 * (half * ks / KS), b1 = min(2 * (half * (ks + 1) / KS), steps);  // never empty
+    constexpr int SB = INT4 ? 2 : 1;  // bytes of a scale
+    const int ring_off = 64 + warp * DEPTH * MV_STAGE_BYTES + lane * 16;
+    const int ring_at = (int)__cvta_generic_to_shared(dyn) + ring_off, at_words = ring_at - lane * 12 + 2048;
+    const uint8_t* s_last = static_cast<const uint8_t*>(a.scales) + (size_t)a.n_mats * a.N * SG * SB - 4;  // last whole word
+    const bool quad_b = (g & 3) == t;  // lanes of the block diagonal of B
 
-    auto mat_of = [&](int li) { return a.ids ? s_ids[s_lead[li]] : 0; };
-    auto load = [&](MvStep (&u)[MV_UB], int mat, int tile, int unit) {
-        const int row = tile * MV_TILE + g;
-        const long long r_lo = (long long)mat * a.N + row;
-        const bool ok_lo = row < a.N, ok_hi = row + 8 < a.N;
-#pragma unroll
-        for (int i = 0; i < MV_UB; i++) {
-            const int b = b0 + unit * MV_UB + i, grp = b * 4 + t, sg = b * 4 + 2 * (t & 1);
-            const uint32_t none = INT4 ? 0x88888888u : 0u;  // codes of zero
-            u[i].lo = u[i].hi = make_uint4(none, none, none, none);
-            u[i].s_lo = u[i].s_hi = 0;
-            if (b < b1 && grp < G) {
-                const uint4* c = reinterpret_cast<const uint4*>(a.codes) + r_lo * G + grp;
-                if (ok_lo)
-                    u[i].lo = __ldcs(c);
-                if (ok_hi)
-                    u[i].hi = __ldcs(c + 8 * (long long)G);
+    int buf = 0;
+    for (int item = i0; item < i1;) {
+        // a run of tiles of one matrix for the same rows of x
+        const int li = item / a.n_tiles, ta = item % a.n_tiles, tb = min(a.n_tiles, ta + i1 - item);
+        item += tb - ta;
+        const int mat = a.ids ? s_ids[s_lead[li]] : 0;
+        const uint8_t* codes = a.codes + (size_t)mat * a.N * G * 16;
+        const uint8_t* scales = static_cast<const uint8_t*>(a.scales) + (size_t)mat * a.N * SG * SB;
+        const int n_mine = ta + slot < tb ? (tb - ta - slot + n_slots - 1) / n_slots : 0;
+
+
+
+
+        // The codes run DEPTH - 1 stages ahead, into the next tile too.  Rows past the end read the last row (and
+        // are not stored); groups past the end are not loaded: what the stage held is finite, and their x is zero.
+        const int g_end = min(G, b1 * 4);
+        int l_left = n_mine * ((b1 - b0 + 1) >> 1), l_tile = ta + slot, l_g = b0 * 4 + t, l_stage = 0;
+        const uint8_t *c_lo, *c_hi, *w_lo_at, *w_hi_at;
+        auto start_tile = [&]() {
+            const int r_lo = min(l_tile * MV_TILE + g, a.N - 1), r_hi = min(l_tile * MV_TILE + g + 8, a.N - 1);
+            c_lo = codes + (size_t)r_lo * G * 16 + (b0 * 4 + t) * 16;
+            c_hi = codes + (size_t)r_hi * G * 16 + (b0 * 4 + t) * 16;
+            l_g = b0 * 4 + t;
+            if (SH != MV_DIRECT) {  // lane t copies word t
+                w_lo_at = scales + ((size_t)r_lo * SG + ((b0 * 4) >> SH)) * SB;
+                w_hi_at = scales + ((size_t)r_hi * SG + ((b0 * 4) >> SH)) * SB;
+                w_lo_at += 4 * t - (reinterpret_cast<uintptr_t>(w_lo_at) & 3);
+                w_hi_at += 4 * t - (reinterpret_cast<uintptr_t>(w_hi_at) & 3);
             }
-            if (b < b1 && sg < G) {
-                if (ok_lo)
-                    u[i].s_lo = mv_load_scales<INT4>(a.scales, r_lo * SG, sg, G, a.group_shift, paired);
-                if (ok_hi)
-                    u[i].s_hi = mv_load_scales<INT4>(a.scales, (r_lo + 8) * SG, sg, G, a.group_shift, paired);
+        };
+        auto load = [&]() {
+            if (l_left > 0) {
+                const int at = ring_at + l_stage;
+                if (l_g < g_end) {
+                    mv_copy16(at, c_lo);
+                    mv_copy16(at + 512, c_hi);
+                }
+                if (l_g + 4 < g_end) {
+                    mv_copy16(at + 1024, c_lo + 64);
+                    mv_copy16(at + 1536, c_hi + 64);
+                }
+                if (SH != MV_DIRECT) {
+                    // what these words hold behind the scales of the stage is not used
+                    const bool mine = t < (INT4 ? (SH == 0 ? 4 : SH == 1 ? 3 : 2) : 3);
+                    if (mine && w_lo_at <= s_last)
+                        mv_copy4(at_words + l_stage, w_lo_at);
+                    if (mine && w_hi_at <= s_last)
+                        mv_copy4(at_words + l_stage + 128, w_hi_at);
+                    w_lo_at += (8 * SB) >> SH;
+                    w_hi_at += (8 * SB) >> SH;
+                }
+                c_lo += 128;
+                c_hi += 128;
+                l_g += 8;
+                l_left--;
+                if (l_g - t >= b1 * 4) {
+                    l_tile += n_slots;
+                    start_tile();
+                }
             }
+            l_stage = l_stage == (DEPTH - 1) * MV_STAGE_BYTES ? 0 : l_stage + MV_STAGE_BYTES;
+            mv_copies_commit();
+        };
+        start_tile();
+#pragma unroll 1
+        for (int i = 0; i < DEPTH - 1; i++)
+            load();
+
+        // the rows of this pass, their x in fp16 and its scales
+        int cnt;
+        __syncthreads();  // the previous run has been computed
+        if (a.ids) {
+            const int first = s_rank[s_lead[li]];
+            const bool in = tid < a.R && s_ids[tid] == mat && s_rank[tid] >= first && s_rank[tid] < first + RP;
+            if (in)
+                s_rows[s_rank[tid] - first] = tid;
+            cnt = __syncthreads_count(in);
+        } else {
+            cnt = min(RP, a.R - li * RP);
+            if (tid < cnt)
+                s_rows[tid] = li * RP + tid;
+            __syncthreads();
         }
-    };
-
-    int li = i0 / a.n_tiles, tile = i0 % a.n_tiles;
-    MvStep cur[MV_UB], nxt[MV_UB];
-    if (i0 < i1)
-        load(cur, mat_of(li), tile, 0);
-
-    int cnt = 0, cur_lead = -1, buf = 0;
-    for (int item = i0; item < i1; item++) {
-        const int mat = mat_of(li);
-        const int li_next = tile + 1 == a.n_tiles ? li + 1 : li, tile_next = tile + 1 == a.n_tiles ? 0 : tile + 1;
-        if (li != cur_lead) {
-            // the rows of this pass, their x in fp16 and its scales
-            cur_lead = li;
-            __syncthreads();  // the previous pass has been computed
-            if (a.ids) {
-                const int first = s_rank[s_lead[li]], same = s_ids[s_lead[li]];
-                const bool in = tid < a.R && s_ids[tid] == same && s_rank[tid] >= first && s_rank[tid] < first + RP;
-                if (in)
-                    s_rows[s_rank[tid] - first] = tid;
-                cnt = __syncthreads_count(in);
-            } else {
-                cnt = min(RP, a.R - li * RP);
-                if (tid < cnt)
-                    s_rows[tid] = li * RP + tid;
-                __syncthreads();
-            }
-            const int chunks = steps * 16;  // of 8 columns; four lanes make a group
-            for (int i = tid; i < cnt * chunks; i += MV_THREADS) {
-                const int c = i / chunks, k8 = i % chunks, grp = k8 >> 2;
-                const long long xr = s_rows[c] / a.rows_per_x;
-                float v[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    v[e] = 0.f;
+        for (int c = 0; c < cnt; c++) {
+            const long long xr = s_rows[c] / a.rows_per_x;
+            for (int k8 = tid; k8 < steps * 16; k8 += MV_THREADS) {  // eight columns; four lanes make a group
+                const int grp = k8 >> 2;
                 float sc = 0.f;
                 uint32_t h[4] = {0, 0, 0, 0};
                 if (grp < G) {
@@ -306,12 +377,12 @@ __global__ void __launch_bounds__(MV_THREADS, 2) w4_matvec_kernel(const MatvecAr
                     h[2] = p2;
                     h[3] = p3;
                 }
-                reinterpret_cast<uint4*>(xs)[c * chunks + k8] = make_uint4(h[0], h[1], h[2], h[3]);
+                xs[c * steps * 16 + k8] = make_uint4(h[0], h[1], h[2], h[3]);
                 if ((k8 & 3) == 0)
                     xsc[c * steps * 4 + grp] = sc;
             }
-            __syncthreads();
         }
+        __syncthreads();
 
         float acc[P][4];
 #pragma unroll
@@ -319,100 +390,142 @@ __global__ void __launch_bounds__(MV_THREADS, 2) w4_matvec_kernel(const MatvecAr
 #pragma unroll
             for (int k = 0; k < 4; k++)
                 acc[p][k] = 0.f;
-
-        for (int unit = 0; unit < units; unit++) {
-            const bool last = unit + 1 == units;
-            if (!last)
-                load(nxt, mat, tile, unit + 1);
-            else if (item + 1 < i1)
-                load(nxt, mat_of(li_next), tile_next, 0);
-#pragma unroll
-            for (int i = 0; i < MV_UB; i++) {
-                const int b = b0 + unit * MV_UB + i;
-                if (b >= b1)
-                    break;
-                float d[P][4];
-#pragma unroll
-                for (int p = 0; p < P; p++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        d[p][k] = 0.f;
-                const uint32_t w_lo[4] = {cur[i].lo.x, cur[i].lo.y, cur[i].lo.z, cur[i].lo.w};
-                const uint32_t w_hi[4] = {cur[i].hi.x, cur[i].hi.y, cur[i].hi.z, cur[i].hi.w};
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    uint32_t l[4], h[4];
-                    mv_decode<INT4>(w_lo[k], l);
-                    mv_decode<INT4>(w_hi[k], h);
-#pragma unroll
-                    for (int p = 0; p < P; p++) {
-                        if (2 * p >= cnt)
-                            break;
-                        uint4 x = make_uint4(0, 0, 0, 0);
-                        const int c = 2 * p + (g >> 2);
-                        if ((g & 3) == t && c < cnt)
-                            x = reinterpret_cast<const uint4*>(xs)[(c * steps + b) * 16 + t * 4 + k];
-                        mv_mma(d[p], l[0], h[0], l[1], h[1], x.x, x.y);
-                        mv_mma(d[p], l[2], h[2], l[3], h[3], x.z, x.w);
-                    }
-                }
-                const float sl0 = mv_scale<INT4>(INT4 ? cur[i].s_lo & 0xFFFFu : cur[i].s_lo & 0xFFu);
-                const float sl1 = mv_scale<INT4>(INT4 ? cur[i].s_lo >> 16 : cur[i].s_lo >> 8);
-                const float sh0 = mv_scale<INT4>(INT4 ? cur[i].s_hi & 0xFFFFu : cur[i].s_hi & 0xFFu);
-                const float sh1 = mv_scale<INT4>(INT4 ? cur[i].s_hi >> 16 : cur[i].s_hi >> 8);
-#pragma unroll
-                for (int p = 0; p < P; p++) {
-                    const int c = 2 * p + (t >> 1);
-                    if (c < cnt) {  // the product with the x scale first: the two scales alone may leave fp32
-                        const float2 sx = *reinterpret_cast<const float2*>(xsc + (c * steps + b) * 4 + 2 * (t & 1));
-                        acc[p][0] = fmaf(d[p][0] * sx.x, sl0, acc[p][0]);
-                        acc[p][1] = fmaf(d[p][1] * sx.y, sl1, acc[p][1]);
-                        acc[p][2] = fmaf(d[p][2] * sx.x, sh0, acc[p][2]);
-                        acc[p][3] = fmaf(d[p][3] * sx.y, sh1, acc[p][3]);
-                    }
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < MV_UB; i++)
-                cur[i] = nxt[i];
-        }
-
-        // rows g and g + 8 of x row 2 p + t / 2: the other two groups are with the neighbouring lane
+        // Lanes off the diagonal, and those of x rows that are not there, read zeros.
+        int x_at[P], x_step[P], sc_at[P];
 #pragma unroll
         for (int p = 0; p < P; p++) {
-            float lo = acc[p][0] + acc[p][1], hi = acc[p][2] + acc[p][3];
-            lo += __shfl_xor_sync(0xffffffffu, lo, 1);
-            hi += __shfl_xor_sync(0xffffffffu, hi, 1);
-            if ((t & 1) == 0) {
-                s_red[buf][warp][g][2 * p + (t >> 1)] = lo;
-                s_red[buf][warp][g + 8][2 * p + (t >> 1)] = hi;
-            }
+            const int c = 2 * p + (g >> 2), cs = 2 * p + (t >> 1);
+            const bool mine = quad_b && c < cnt;
+            x_at[p] = mine ? xs_at + (c * steps * 16 + t * 4) * 16 : 0;
+            x_step[p] = mine ? 256 : 0;
+            sc_at[p] = xsc_at + (min(cs, cnt - 1) * steps * 4 + 2 * (t & 1)) * 4;
         }
-        __syncthreads();
-        if (warp < P) {  // 16 rows x 2 rows of x per warp
-            const int r = tid & 15, c = tid >> 4, n = tile * MV_TILE + r;
-            float v = 0.f;
+        int stage = 0;
+        for (int tile = ta + slot; tile < tb; tile += n_slots) {
+            const uint8_t* s_lo = scales + (size_t)min(tile * MV_TILE + g, a.N - 1) * SG * SB;
+            const uint8_t* s_hi = scales + (size_t)min(tile * MV_TILE + g + 8, a.N - 1) * SG * SB;
+            uint32_t pick_lo = 0, pick_hi = 0;
+            if (SH != MV_DIRECT) {
+                pick_lo = mv_pick<INT4, SH>(s_lo + ((b0 * 4) >> SH) * SB, t);
+                pick_hi = mv_pick<INT4, SH>(s_hi + ((b0 * 4) >> SH) * SB, t);
+            }
+#pragma unroll 1
+            for (int b = b0; b < b1; b += 2) {
+                mv_copies_wait<DEPTH - 2>();
+                __syncwarp();  // every lane's copies have landed, and the stage before this one has been read
+                load();
+                const uint8_t* st = dyn + ring_off + stage;
+                uint4 words_lo, words_hi;
+                if (SH != MV_DIRECT) {
+                    const uint8_t* sw = dyn + ring_off - lane * 16 + 2048 + g * 16 + stage;
+                    words_lo = *reinterpret_cast<const uint4*>(sw);
+                    words_hi = *reinterpret_cast<const uint4*>(sw + 128);
+                }
 #pragma unroll
-            for (int w = 0; w < MV_WARPS; w++)
-                v += s_red[buf][w][r][c];
-            if (!INT4)
-                v *= 2.f;  // mv_scale
-            if (a.bias && n < a.N)
-                v += a.bias[(long long)mat * a.N + n];
-            const float up = __shfl_down_sync(0xffffffffu, v, 1);
-            if (c < cnt && n < a.N) {
-                const long long row = (long long)s_rows[c] * a.out_stride;
-                if (!a.swiglu) {
-                    store_from_float(a.out, row + n, a.out_dtype, v);
-                } else if ((r & 1) == 0) {
-                    const float gt = fminf(v, a.limit), u = fminf(fmaxf(up, -a.limit), a.limit);
-                    store_from_float(a.out, row + (n >> 1), a.out_dtype, gt / (1.f + expf(-a.alpha * gt)) * (u + 1.f));
+                for (int h = 0; h < 2; h++) {
+                    const uint4 c_lo4 = *reinterpret_cast<const uint4*>(st + h * 1024);
+                    const uint4 c_hi4 = *reinterpret_cast<const uint4*>(st + h * 1024 + 512);
+                    const uint32_t w_lo[4] = {c_lo4.x, c_lo4.y, c_lo4.z, c_lo4.w};
+                    const uint32_t w_hi[4] = {c_hi4.x, c_hi4.y, c_hi4.z, c_hi4.w};
+                    uint32_t l[4][4], u[4][4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        mv_decode<INT4>(w_lo[k], l[k]);
+                        mv_decode<INT4>(w_hi[k], u[k]);
+                    }
+                    uint32_t raw_lo, raw_hi;
+                    if (SH != MV_DIRECT) {
+                        raw_lo = mv_from_words<INT4, SH>(words_lo, pick_lo, h);
+                        raw_hi = mv_from_words<INT4, SH>(words_hi, pick_hi, h);
+                        if ((b + h) * 4 + 4 > g_end) {  // what lies behind the last scale is not this row's, and may be NaN
+                            const int left = g_end - (b + h) * 4 - 2 * (t & 1);
+                            const uint32_t own = left > 1 ? 0xFFFFFFFFu : left == 1 ? (INT4 ? 0xFFFFu : 0xFFu) : 0u;
+                            raw_lo &= own;
+                            raw_hi &= own;
+                        }
+                    } else {
+                        raw_lo = mv_load_scales<INT4>(s_lo, (b + h) * 4 + 2 * (t & 1), g_end, a.group_shift);
+                        raw_hi = mv_load_scales<INT4>(s_hi, (b + h) * 4 + 2 * (t & 1), g_end, a.group_shift);
+                    }
+                    const float2 w_s_lo = mv_scales<INT4>(raw_lo), w_s_hi = mv_scales<INT4>(raw_hi);
+                    // The second step of the last stage may not be this warp's: its x counts as zero.
+                    const bool there = h == 0 || b + 1 < b1;
+#pragma unroll
+                    for (int p = 0; p < P; p++) {
+                        if (P > 1 && 2 * p >= cnt)
+                            break;
+                        const uint4* x = reinterpret_cast<const uint4*>(dyn + (there ? x_at[p] + x_step[p] * (b + h) : 0));
+                        const uint4 x0 = x[0], x1 = x[1], x2 = x[2], x3 = x[3];
+                        float d[4];
+                        mv_mma_first(d, l[0][0], u[0][0], l[0][1], u[0][1], x0.x, x0.y);
+                        mv_mma(d, l[0][2], u[0][2], l[0][3], u[0][3], x0.z, x0.w);
+                        mv_mma(d, l[1][0], u[1][0], l[1][1], u[1][1], x1.x, x1.y);
+                        mv_mma(d, l[1][2], u[1][2], l[1][3], u[1][3], x1.z, x1.w);
+                        mv_mma(d, l[2][0], u[2][0], l[2][1], u[2][1], x2.x, x2.y);
+                        mv_mma(d, l[2][2], u[2][2], l[2][3], u[2][3], x2.z, x2.w);
+                        mv_mma(d, l[3][0], u[3][0], l[3][1], u[3][1], x3.x, x3.y);
+                        mv_mma(d, l[3][2], u[3][2], l[3][3], u[3][3], x3.z, x3.w);
+                        // the product with the x scale first: the two scales alone may leave fp32
+                        const float2 sx = *reinterpret_cast<const float2*>(dyn + (there ? sc_at[p] + 16 * (b + h) : 0));
+                        acc[p][0] = fmaf(d[0] * sx.x, w_s_lo.x, acc[p][0]);
+                        acc[p][1] = fmaf(d[1] * sx.y, w_s_lo.y, acc[p][1]);
+                        acc[p][2] = fmaf(d[2] * sx.x, w_s_hi.x, acc[p][2]);
+                        acc[p][3] = fmaf(d[3] * sx.y, w_s_hi.y, acc[p][3]);
+                    }
+                }
+                stage = stage == (DEPTH - 1) * MV_STAGE_BYTES ? 0 : stage + MV_STAGE_BYTES;
+            }
+
+            // the end of a tile: rows g and g + 8 of x row 2 p + t / 2, two groups here, two with lane t ^ 1
+            float lo[P], hi[P];
+#pragma unroll
+            for (int p = 0; p < P; p++) {
+                lo[p] = acc[p][0] + acc[p][1];
+                hi[p] = acc[p][2] + acc[p][3];
+                lo[p] += __shfl_xor_sync(0xffffffffu, lo[p], 1);
+                hi[p] += __shfl_xor_sync(0xffffffffu, hi[p], 1);
+                acc[p][0] = acc[p][1] = acc[p][2] = acc[p][3] = 0.f;
+            }
+            if (KS > 1) {
+                if (ks > 0 && (t & 1) == 0)
+#pragma unroll
+                    for (int p = 0; p < P; p++)
+                        s_red[buf][warp][p][lane >> 1] = make_float2(lo[p], hi[p]);
+                asm volatile("bar.sync %0, %1;" ::"r"(1 + slot), "r"(32 * KS) : "memory");
+                if (ks == 0)
+                    for (int w = 1; w < KS; w++)
+#pragma unroll
+                        for (int p = 0; p < P; p++) {
+                            const float2 v = s_red[buf][warp + w][p][lane >> 1];
+                            lo[p] += v.x;
+                            hi[p] += v.y;
+                        }
+                buf ^= 1;
+            }
+            if (ks == 0) {
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const int n = tile * MV_TILE + g + 8 * half;
+                    const float bias = a.bias && n < a.N ? a.bias[(size_t)mat * a.N + n] : 0.f;
+#pragma unroll
+                    for (int p = 0; p < P; p++) {
+                        const float v = (half ? hi[p] : lo[p]) + bias;
+                        const float up = __shfl_down_sync(0xffffffffu, v, 4);  // row g + 1
+                        const int c = 2 * p + (t >> 1);
+                        if ((t & 1) == 0 && c < cnt && n < a.N) {
+                            const long long row = (long long)s_rows[c] * a.out_stride;
+                            if (!a.swiglu) {
+                                store_from_float(a.out, row + n, a.out_dtype, v);
+                            } else if ((g & 1) == 0) {
+                                const float gt = v > a.limit ? a.limit : v;  // comparisons that let NaN through
+                                const float u = up > a.limit ? a.limit : up < -a.limit ? -a.limit : up;
+                                store_from_float(a.out, row + (n >> 1), a.out_dtype, gt / (1.f + expf(-a.alpha * gt)) * (u + 1.f));
+                            }
+                        }
+                    }
                 }
             }
         }
-        buf ^= 1;
-        li = li_next;
-        tile = tile_next;
     }
 
     // rows without a matrix

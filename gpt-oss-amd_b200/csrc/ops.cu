@@ -16,6 +16,7 @@ using namespace moe::op;
 namespace {
 
 constexpr int MAX_DEVICES = 64;
+constexpr size_t MV_MAX_SMEM = 212 * 1024;  // dynamic shared memory of w4_matvec_kernel
 
 moe_b200_status refuse(moe_b200_status st, const char* fmt, ...) {
     va_list ap;
@@ -259,22 +260,37 @@ moe_b200_status moe_b200_w4_matvec(const moe_b200_w4_matrix* w, const void* x, i
     a.out_stride = out_stride;
     a.out_dtype = out_dtype;
     a.n_tiles = (N + MV_TILE - 1) / MV_TILE;
+    a.ksplit = a.n_tiles < 1024 ? 4 : 2;  // by the matrix alone: a row's sums have one order in every batch
+    while (a.ksplit > (mv_steps(K) + 1) / 2)
+        a.ksplit /= 2;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
 
-    // rows of x per pass over the weights: 2, 4 or 8, as many as there are and shared memory holds
-    int pairs = n_rows <= 2 ? 1 : n_rows <= 4 ? 2 : 4;
-    while (pairs > 1 && mv_smem_bytes(K, 2 * pairs) > 200 * 1024)
+    // Pairs of x rows per pass over the weights.  Chosen matrices are shared by n_rows / n_mats rows on the average.
+    const int share = ids ? (n_rows + w->n_mats - 1) / w->n_mats : n_rows;
+    int pairs = share <= 2 ? 1 : share <= 4 ? 2 : 4;
+    auto smem_of = [&](int p) { return mv_smem_bytes(K, p, n_rows < 2 * p ? n_rows : 2 * p); };
+    while (pairs > 1 && smem_of(pairs) > MV_MAX_SMEM)
         pairs /= 2;
-    const size_t smem = mv_smem_bytes(K, 2 * pairs);
-    auto kernel = int4 ? (pairs == 1 ? w4_matvec_kernel<true, 1> : pairs == 2 ? w4_matvec_kernel<true, 2> : w4_matvec_kernel<true, 4>)
-                       : (pairs == 1 ? w4_matvec_kernel<false, 1> : pairs == 2 ? w4_matvec_kernel<false, 2> : w4_matvec_kernel<false, 4>);
+    const size_t smem = smem_of(pairs);
+    const long long scale_bytes = (long long)w->n_mats * N * (K / w->group) * (int4 ? 2 : 1);
+    const bool words = !(int4 && w->group == 32 && (K / 32) % 2) && aligned(w->scales, 4) && scale_bytes % 4 == 0;
+    const int sh = words ? a.group_shift : MV_DIRECT;
+    typedef void (*Kernel)(MatvecArgs);
+#define MV_ROW(I4, S) {w4_matvec_kernel<I4, S, 1>, w4_matvec_kernel<I4, S, 2>, w4_matvec_kernel<I4, S, 4>}
+    static const Kernel kernels[2][4][3] = {
+        {MV_ROW(false, 0), {nullptr, nullptr, nullptr}, {nullptr, nullptr, nullptr}, MV_ROW(false, MV_DIRECT)},
+        {MV_ROW(true, 0), MV_ROW(true, 1), MV_ROW(true, 2), MV_ROW(true, MV_DIRECT)}};
+#undef MV_ROW
+    const Kernel kernel = kernels[int4][sh][pairs >> 1];
     if (smem > 32 * 1024) {  // with the fixed part more than a block has without asking
-        cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+        cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, MV_MAX_SMEM);
         if (e != cudaSuccess)
             return launched("moe_b200_w4_matvec: shared memory", e);
     }
     const long long passes = ids ? n_rows : (n_rows + 2 * pairs - 1) / (2 * pairs);
-    const long long items = passes * a.n_tiles, most = (smem > 90 * 1024 ? 1 : 2) * (long long)sms;
+    const int fixed = 1024 + 2048 + 64 + 2 * pairs * 4 + pairs * 2048 + 1024;  // static shared memory and the system's
+    const long long fit = (228 * 1024) / ((long long)smem + fixed), occ = MV_BLOCKS;
+    const long long items = passes * a.n_tiles, most = (fit < 1 ? 1 : fit < occ ? fit : occ) * sms;
     kernel<<<(unsigned)(items < most ? items : most), MV_THREADS, smem, st>>>(a);
     return launched("moe_b200_w4_matvec", cudaGetLastError());
 }

@@ -457,8 +457,8 @@ moe_b200_status moe_b200_route_logits(const void* logits, int dtype, long long s
 /* A stack of matrices in 4 bits.  Two codes per byte, the even column in the low
  * half; codes 16-byte aligned.
  *   MXFP4  e2m1 codes, scales e8m0 bytes per group of 32 (checkpoint layout: the
- *          blocks and scales of moe_b200_set_experts_mxfp4), value 2^(byte - 127)
- *          for every byte
+ *          blocks and scales of moe_b200_set_experts_mxfp4), value 2^(byte - 127);
+ *          byte 255 is NaN, as the MX format defines it
  *   INT4   value code - 8, scales bf16 per group of 32, 64 or 128 */
 #define MOE_B200_W4_MXFP4 0
 #define MOE_B200_W4_INT4 1
@@ -488,7 +488,7 @@ typedef struct {
  * Products are exact and summed in fp32; one rounding at the end.  Row addresses
  * of x must be 16-byte aligned (8 bytes for e4m3). */
 #define MOE_B200_W4_MATVEC_MAX_ROWS 256
-#define MOE_B200_W4_MATVEC_MAX_IN 32768
+#define MOE_B200_W4_MATVEC_MAX_IN 16384
 #define MOE_B200_W4_MATVEC_MAX_OUT 4194304
 moe_b200_status moe_b200_w4_matvec(const moe_b200_w4_matrix* w, const void* x, int x_dtype, long long x_stride,
                                    const void* x_scales, int x_scale_kind, int n_rows, int rows_per_x, const int* ids,

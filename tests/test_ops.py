@@ -318,8 +318,8 @@ def _check_matvec(got, x64, codes, scales, bias, group, ids, rpx, swiglu=None, l
     (16, 32, 1, "mxfp4", 32, BF16, F32, False), (1, 64, 1, "mxfp4", 32, F16, F32, True), (17, 96, 2, "mxfp4", 32, "mx", BF16, True),
     (33, 160, 3, "int4", 32, BF16, F16, True), (48, 128, 5, "int4", 128, "row", F32, False), (100, 320, 8, "int4", 64, 64, F32, True),
     (2880, 2880, 1, "mxfp4", 32, BF16, F32, True), (5120, 2880, 2, "mxfp4", 32, "mx", F32, False), (2881, 2848, 4, "mxfp4", 32, 128, F32, True),
-    (515, 4096, 7, "int4", 128, F16, F32, True), (96, 8192, 9, "mxfp4", 32, 32, F32, False), (31, 32768, 3, "mxfp4", 32, BF16, F32, True),
-    (64, 32768, 8, "int4", 64, "row", F32, True), (64, 1024, 17, "mxfp4", 32, BF16, F32, True), (40, 1056, 256, "int4", 32, F16, F32, True),
+    (515, 4096, 7, "int4", 128, F16, F32, True), (96, 8192, 9, "mxfp4", 32, 32, F32, False), (31, 16384, 3, "mxfp4", 32, BF16, F32, True),
+    (64, 16384, 8, "int4", 64, "row", F32, True), (64, 1024, 17, "mxfp4", 32, BF16, F32, True), (40, 1056, 256, "int4", 32, F16, F32, True),
     (20000, 512, 1, "int4", 64, BF16, F32, False)])
 def test_w4_matvec(N, K, M, fmt, group, kind, out, bias):
     g = _gen(N + K + M)
@@ -380,7 +380,7 @@ def test_w4_matvec_checkpoint_blocks_and_every_code():
 
 
 def test_w4_matvec_every_scale_byte():
-    """Each e8m0 byte is 2^(byte - 127), 255 included, as in mxfp4_unpack; exact while fp32 holds the result."""
+    """Each e8m0 byte is 2^(byte - 127), exact while fp32 holds the result; 255 is NaN, as the format has it."""
     N, K = 256, 32
     scales = torch.arange(256, device="cuda").to(torch.uint8).view(N, 1)
     codes = torch.zeros(N, K // 2, dtype=torch.uint8, device="cuda")
@@ -389,13 +389,15 @@ def test_w4_matvec_every_scale_byte():
         x = torch.zeros(1, K, dtype=BF16, device="cuda")
         x[0, 0] = v
         y = pkg.w4_matvec(x, codes, scales, dtype=F32)[0].double()
-        want = (torch.arange(256, device="cuda").double() - 127).exp2() * v
+        assert y[255].isnan()
+        y = y[:255]
+        want = (torch.arange(255, device="cuda").double() - 127).exp2() * v
         inside = (want < 2.0**128) & (want >= 2.0**-149)
         assert torch.equal(y[inside], want[inside])
         assert (y[want >= 2.0**128] == math.inf).all()
     # codes of zero stay zero under the largest scale
     codes[:, 0] = 0
-    assert (pkg.w4_matvec(torch.ones(1, K, dtype=BF16, device="cuda"), codes, scales, dtype=F32) == 0).all()
+    assert (pkg.w4_matvec(torch.ones(1, K, dtype=BF16, device="cuda"), codes, scales, dtype=F32)[0, :255] == 0).all()
 
 
 @pytest.mark.parametrize("mag", [1e-30, 1e-6, 1.0, 1e6, 1e30])
@@ -424,6 +426,8 @@ def test_w4_matvec_infinity_and_nan_stay_in_their_row():
     w = ref.dequant(codes, scales, 32)[:, 40]
     assert y[2][w == 0].isnan().all()
     assert (y[2][w != 0].double() == w[w != 0].sign() * math.inf).all()
+    act = pkg.w4_matvec(x, codes, scales, swiglu=(1.702, 7.0), dtype=F32)
+    assert act[1].isnan().all() and not act[[0, 3]].isnan().any()  # the clamps of the SwiGLU keep NaN
 
 
 def test_w4_matvec_one_x_for_all_rows_and_strided_rows():

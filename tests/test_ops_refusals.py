@@ -57,7 +57,7 @@ def test_route_logits_refuses(kw):
 
 @pytest.mark.parametrize("mat,kw", [
     (dict(format=2), {}), (dict(group=64), {}), (dict(format=1, group=16), {}), (dict(rows=0), {}), (dict(rows=4194305), {}),
-    (dict(cols=0), {}), (dict(cols=48), {}), (dict(cols=32800), {}), (dict(format=1, group=128), {}), (dict(n_mats=0), {}),
+    (dict(cols=0), {}), (dict(cols=48), {}), (dict(cols=16416), {}), (dict(format=1, group=128), {}), (dict(n_mats=0), {}),
     (dict(n_mats=2), {}), (dict(codes=None), {}), (dict(scales=None), {}), (dict(codes=A + 8), {}), (dict(bias=A + 2), {}),
     (dict(format=1, scales=A + 1), {}),
     ({}, dict(M=-1)), ({}, dict(M=257)), ({}, dict(rpx=0)), ({}, dict(xt=capi.DTYPE_F32)), ({}, dict(xt=capi.DTYPE_E4M3)),
