@@ -7,15 +7,21 @@
 //
 // The indices are whole numbers and must not depend on a rounding: their order is that of keys in
 // 64 bits.  Logits order exactly as they are.  Keys that are sums are computed in fp32 first, and
-// a warp whose decision hung on a gap below the fp32 error does its token again with
-// 64-bit keys (route_select<double>): about one token in a hundred for fp32 logits.  The weights of
-// the K selected come from 64-bit exponentials, one lane each.
+// a warp whose decision hung on a gap below the fp32 error ranks those that may be among the K by
+// 64-bit keys, a few tokens in a thousand for fp32 logits; where it hung on the groups, or on more
+// than 32 experts, it does the token again in 64 bits (route_exact).
 //
 // A warp owns a token; lane i holds the NT neighbouring experts from i * NT on, so the lowest
-// lane of a tie has the lowest index.  K rounds of a warp-wide maximum.  Bound by the latency of
-// that chain for few tokens and by instruction issue for many; the logits are read once.
+// lane of a tie has the lowest index.  Each lane sorts its keys once (a network of 19 exchanges for
+// 8); then a round per selected expert takes the largest of the 32 heads (one warp reduction) and
+// the winner moves on to its next key.  The logits are read once, 16 bytes a lane where they
+// are aligned.  Bound by instruction issue for many tokens, by the latency of the
+// rounds for few.
 #pragma once
 #include <float.h>
+
+#include <type_traits>
+#include <utility>
 
 #include "op_types.cuh"
 
@@ -59,201 +65,479 @@ __device__ __forceinline__ F warp_sum(F v) {
     return v;
 }
 
-__device__ __forceinline__ float exp_of(float x) { return expf(x); }
-__device__ __forceinline__ double exp_of(double x) { return exp(x); }
-
-// Largest key of the warp and the lowest expert that has it.  Keys never hold NaN.
-__device__ __forceinline__ float warp_best(float v, int& e) {
-    // floats as integers of the same order; -inf stays below everything
-    const uint32_t b = __float_as_uint(v + 0.f);  // -0 counts as +0
-    const uint32_t u = b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
-    const uint32_t top = __reduce_max_sync(0xffffffffu, u);
-    e = __shfl_sync(0xffffffffu, e, __ffs(__ballot_sync(0xffffffffu, u == top)) - 1);
-    return __uint_as_float(top ^ ((top >> 31) ? 0x80000000u : 0xFFFFFFFFu));
-}
-__device__ __forceinline__ double warp_best(double v, int& e) {
-    const double top = warp_max(v);
-    e = __shfl_sync(0xffffffffu, e, __ffs(__ballot_sync(0xffffffffu, v == top)) - 1);
-    return top;
+// Largest value of the warp.  Keys never hold NaN.
+__device__ __forceinline__ float warp_best(float v) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
 }
 
-// One token.  l[j]: logit of expert lane * NT + j, -inf where it takes no part.  `keys`: E values of
-// shared memory of this warp (group scores).  sel[k] in every lane; returns false where an fp32
-// decision was too close to call.  sum: the softmax's (0 where nothing needs it).
-template <typename F, int NT>
-__device__ __forceinline__ bool route_select(const LogitsArgs& a, const float (&l)[NT], float lmax, F* keys, int lane,
-                                             int* sel, F& sum) {
-    // Without a bias the logits are the keys of the experts, and of groups scored by their best.
-    const bool by_logit = a.bias == nullptr;
-    const bool need_p = !by_logit || (a.n_groups > 1 && a.group_top > 1);
-    F p[NT];
-    sum = 0;
-    if (!a.sigmoid && (need_p || !a.renorm)) {
-#pragma unroll
-        for (int j = 0; j < NT; j++) {
-            p[j] = l[j] > -INFINITY ? exp_of((F)l[j] - (F)lmax) : (F)0;
-            sum += p[j];
+// The logit that takes part: NaN and -inf do not (-inf), +inf is the largest finite value.
+__device__ __forceinline__ float route_logit(float v) { return v > -INFINITY ? fminf(v, FLT_MAX) : -INFINITY; }
+
+// One token with 64-bit keys, from the definition and without hurry: `keys` holds E values of shared memory of
+// this warp.  Returns the expert of slot `lane`, -1 where there is none.
+__device__ __noinline__ int route_exact(const LogitsArgs& a, long long t, float lmax, double* keys, int lane) {
+    const long long at = t * a.stride;
+    double sum = 0.0;
+    if (!a.sigmoid)
+        for (int e = lane; e < a.E; e += 32) {
+            const float l = route_logit(load_as_float(a.logits, at + e, a.dtype));
+            if (l > -INFINITY)
+                sum += exp((double)l - (double)lmax);
         }
-        sum = warp_sum(sum);
-    }
-    if (need_p) {
-#pragma unroll
-        for (int j = 0; j < NT; j++) {
-            if (a.sigmoid)
-                p[j] = l[j] > -INFINITY ? (F)1 / ((F)1 + exp_of(-(F)l[j])) : (F)0;
-            else
-                p[j] = p[j] / sum;
+    sum = warp_sum(sum);
+    for (int e = lane; e < a.E; e += 32) {
+        const float l = route_logit(load_as_float(a.logits, at + e, a.dtype));
+        const float b = a.bias ? a.bias[e] : 0.f;
+        double p = -INFINITY;
+        if (l > -INFINITY && b > -INFINITY) {
+            p = a.sigmoid ? 1.0 / (1.0 + exp(-(double)l)) : exp((double)l - (double)lmax) / sum;
+            p += (double)fminf(b, FLT_MAX);
         }
+        keys[e] = p;  // without a bias p itself: the groups' scores
     }
-    // Two fp32 keys closer than this may be in the other order in 64 bits: p is off by up to 48
-    // half steps of its size (the exponential's two steps, the rounded difference in its argument, the
-    // sum of up to 512 terms in a tree, the division), p + bias by half a step of the sum's.
-    constexpr bool check = sizeof(F) == 4;
-    constexpr float TOL = 2.f * 49.f * 5.97e-8f;
-    bool sure = true;
-    F key[NT];
-#pragma unroll
-    for (int j = 0; j < NT; j++) {
-        const int e = lane * NT + j;
-        key[j] = -INFINITY;
-        if (l[j] > -INFINITY) {
-            const float b = by_logit ? 0.f : a.bias[e];
-            key[j] = by_logit ? (F)l[j] : b > -INFINITY ? p[j] + (F)fminf(b, FLT_MAX) : (F)-INFINITY;
-        }
-    }
+    __syncwarp();
+    unsigned kept = 0xffffffffu;
+    const int gs = a.E / a.n_groups;
     if (a.n_groups > 1) {
-        // a group's score by the lane of its number
-        const int gs = a.E / a.n_groups;
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < NT; j++)
-            if (lane * NT + j < a.E)
-                keys[lane * NT + j] = (by_logit && a.group_top > 1 && l[j] > -INFINITY) ? p[j] : key[j];
-        __syncwarp();
-        F b1 = -INFINITY, b2 = -INFINITY;
+        double b1 = -INFINITY, b2 = -INFINITY;
         if (lane < a.n_groups)
             for (int i = 0; i < gs; i++) {
-                const F v = keys[lane * gs + i];
+                const double v = keys[lane * gs + i];
                 b2 = v > b1 ? b1 : (v > b2 ? v : b2);
                 b1 = v > b1 ? v : b1;
             }
-        F score = b1;
-        if (a.group_top > 1 && b2 > -INFINITY)
-            score += b2;
-        const bool exact = by_logit && a.group_top == 1;
-        unsigned kept = 0;
-        F last = INFINITY;
-        for (int k = 0; k <= a.topk_groups && k < a.n_groups; k++) {
-            int g = lane;
-            const F s = warp_best(score, g);
-            if (k == a.topk_groups) {
-                if (check && !exact && s > -INFINITY)
-                    sure &= (float)(last - s) > 2.f * TOL * fmaxf(1.f, fabsf((float)last));
-            } else if (s > -INFINITY) {
+        double score = a.group_top > 1 && b2 > -INFINITY ? b1 + b2 : b1;
+        kept = 0;
+        for (int k = 0; k < a.topk_groups; k++) {
+            const double top = warp_max(score);
+            const int g = __ffs(__ballot_sync(0xffffffffu, score == top)) - 1;
+            if (top > -INFINITY)
                 kept |= 1u << g;
-                if (lane == g)
-                    score = -INFINITY;
-            }
-            last = s;
-        }
-#pragma unroll
-        for (int j = 0; j < NT; j++) {
-            const int e = lane * NT + j;
-            if (e < a.E && !((kept >> (e / gs)) & 1u))
-                key[j] = -INFINITY;
+            if (lane == g)
+                score = -INFINITY;
         }
     }
-    F last = INFINITY;
-    for (int k = 0; k <= a.K; k++) {
-        F v = key[0];
-        int e = lane * NT;
-#pragma unroll
-        for (int j = 1; j < NT; j++)
-            if (key[j] > v) {
-                v = key[j];
-                e = lane * NT + j;
-            }
-        v = warp_best(v, e);
-        if (check && !by_logit && k > 0 && v > -INFINITY)
-            sure &= (float)(last - v) > TOL * fmaxf(1.f, fabsf((float)last));
-        last = v;
-        if (k < a.K) {
-            if (!(v > -INFINITY))
-                e = -1;
-            if (lane == 0)
-                sel[k] = e;
-#pragma unroll
-            for (int j = 0; j < NT; j++)
-                if (e == lane * NT + j)
-                    key[j] = -INFINITY;
-        } else if (by_logit || !check) {
-            break;
-        }
+    for (int e = lane; e < a.E; e += 32) {
+        if (!((kept >> (e / gs)) & 1u))
+            keys[e] = -INFINITY;
+        else if (!a.bias)  // the logits order the experts
+            keys[e] = route_logit(load_as_float(a.logits, at + e, a.dtype));
     }
     __syncwarp();
-    return sure;
+    int mine = -1;
+    for (int k = 0; k < a.K; k++) {
+        double v = -INFINITY;
+        int e = a.E;
+        for (int i = lane; i < a.E; i += 32)
+            if (keys[i] > v) {
+                v = keys[i];
+                e = i;
+            }
+        const double top = warp_max(v);
+        const int win = (int)__reduce_min_sync(0xffffffffu, v == top ? (unsigned)e : 0xffffffffu);
+        if (!(top > -INFINITY))
+            break;
+        if (lane == k)
+            mine = win;
+        if (lane == (win & 31))
+            keys[win] = -INFINITY;
+        __syncwarp();
+    }
+    return mine;
 }
 
-constexpr int ROUTE_WARPS = 4;
+constexpr int ROUTE_WARPS = 16;
 
+// The exchanges of Batcher's odd-even merge sort of NT places, in order.
 template <int NT>
-__global__ void __launch_bounds__(32 * ROUTE_WARPS) route_logits_kernel(const LogitsArgs a) {
-    __shared__ double s_keys[ROUTE_WARPS][32 * NT];
-    __shared__ int s_sel[ROUTE_WARPS][ROUTE_MAX_K];
-    __shared__ int s_hist[32 * NT];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (a.counts) {
-        for (int i = threadIdx.x; i < a.E; i += blockDim.x)
-            s_hist[i] = 0;
-        __syncthreads();
+struct SortNetwork {
+    int x[NT * NT], y[NT * NT], n;
+    constexpr SortNetwork() : x{}, y{}, n(0) {
+        for (int p = 1; p < NT; p *= 2)
+            for (int k = p; k >= 1; k /= 2)
+                for (int j = k % p; j + k < NT; j += 2 * k)
+                    for (int i = 0; i < k && i + j + k < NT; i++)
+                        if ((i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                            x[n] = i + j;
+                            y[n] = i + j + k;
+                            n++;
+                        }
     }
+};
+
+template <int NT, int... I>
+__device__ __forceinline__ void sort_exchanges(float (&key)[NT], int (&idx)[NT], std::integer_sequence<int, I...>) {
+    constexpr SortNetwork<NT> net;
+    auto exchange = [&](int x, int y) {
+        const bool swap = key[y] > key[x] || (key[y] == key[x] && idx[y] < idx[x]);
+        const float kx = swap ? key[y] : key[x], ky = swap ? key[x] : key[y];
+        const int ix = swap ? idx[y] : idx[x], iy = swap ? idx[x] : idx[y];
+        key[x] = kx;
+        key[y] = ky;
+        idx[x] = ix;
+        idx[y] = iy;
+    };
+    (exchange(std::integral_constant<int, net.x[I]>::value, std::integral_constant<int, net.y[I]>::value), ...);
+}
+
+// Sorts the keys of a lane in falling order, ties by index; perm: four bits per place, the index within the lane.
+template <int NT, typename Perm>
+__device__ __forceinline__ void sort_lane(float (&key)[NT], Perm& perm) {
+    int idx[NT];
+#pragma unroll
+    for (int j = 0; j < NT; j++)
+        idx[j] = j;
+    constexpr SortNetwork<NT> net;
+    sort_exchanges<NT>(key, idx, std::make_integer_sequence<int, net.n>{});
+    perm = 0;
+#pragma unroll
+    for (int j = 0; j < NT; j++)
+        perm |= (Perm)idx[j] << (4 * j);
+}
+
+// VEC: a lane's logits are one aligned piece of memory.
+template <int NT, bool VEC>
+__global__ void __launch_bounds__(32 * ROUTE_WARPS) route_logits_kernel(const __grid_constant__ LogitsArgs a) {
+    typedef typename std::conditional<NT == 16, unsigned long long, unsigned>::type Perm;
+    __shared__ float s_sorted[ROUTE_WARPS][NT + 1][32];  // place, lane
+    __shared__ int s_sel[ROUTE_WARPS][32];
+    extern __shared__ double s_keys_all[];  // [warps][32 * NT]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    double* s_keys = s_keys_all + warp * 32 * NT;
+    if (a.counts && blockIdx.x == 0)
+        for (int i = threadIdx.x; i < a.E; i += blockDim.x)
+            a.counts[i] = 0;  // route_counts_kernel adds to them
+    // Without a bias the logits are the keys of the experts, and of groups that are scored by their best.
+    const bool by_logit = a.bias == nullptr;
+    const bool need_p = !by_logit || (a.n_groups > 1 && a.group_top > 1);
+    const int gs = a.E / a.n_groups, span = gs / NT;  // lanes of a group, where that is a power of two of them
+    const bool lanes_of_group = gs % NT == 0 && (span & (span - 1)) == 0;
+    float bias[NT];
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+        const int e = lane * NT + j;
+        const float b = a.bias && e < a.E ? a.bias[e] : 0.f;
+        bias[j] = b > -INFINITY ? fminf(b, FLT_MAX) : -INFINITY;
+    }
+    float(*sorted)[32] = s_sorted[warp];
+    sorted[NT][lane] = -INFINITY;
+    int* sel = s_sel[warp];
     for (int t = blockIdx.x * (blockDim.x >> 5) + warp; t < a.T; t += gridDim.x * (blockDim.x >> 5)) {
         float l[NT];
+        const long long at = (long long)t * a.stride;
+        if (VEC && lane * NT + NT <= a.E) {
+            if (a.dtype == MOE_B200_DTYPE_F32) {
+                const float* src = static_cast<const float*>(a.logits) + at + lane * NT;
+                if (NT >= 4) {
+#pragma unroll
+                    for (int j = 0; j < NT; j += 4) {
+                        const float4 v = *reinterpret_cast<const float4*>(src + j);
+                        l[j] = v.x, l[(j + 1) % NT] = v.y, l[(j + 2) % NT] = v.z, l[(j + 3) % NT] = v.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < NT; j++)
+                        l[j] = src[j];
+                }
+            } else {
+                const uint16_t* src = static_cast<const uint16_t*>(a.logits) + at + lane * NT;
+                uint32_t w[(NT + 1) / 2];
+                if (NT >= 8) {
+#pragma unroll
+                    for (int j = 0; j < NT / 2; j += 4) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(src + 2 * j);
+                        w[j] = v.x, w[(j + 1) % ((NT + 1) / 2)] = v.y, w[(j + 2) % ((NT + 1) / 2)] = v.z, w[(j + 3) % ((NT + 1) / 2)] = v.w;
+                    }
+                } else if (NT == 4) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(src);
+                    w[0] = v.x, w[1 % ((NT + 1) / 2)] = v.y;
+                } else if (NT == 2) {
+                    w[0] = *reinterpret_cast<const uint32_t*>(src);
+                } else {
+                    w[0] = *src;
+                }
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+                    l[j] = half_to_float((w[j >> 1] >> (16 * (j & 1))) & 0xFFFFu, a.dtype);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                const int e = lane * NT + j;
+                l[j] = e < a.E ? load_as_float(a.logits, at + e, a.dtype) : -INFINITY;
+            }
+        }
         float lmax = -INFINITY;
 #pragma unroll
         for (int j = 0; j < NT; j++) {
-            const int e = lane * NT + j;
-            l[j] = -INFINITY;
-            if (e < a.E) {
-                const float v = load_as_float(a.logits, (long long)t * a.stride + e, a.dtype);
-                l[j] = v > -INFINITY ? fminf(v, FLT_MAX) : -INFINITY;  // NaN compares false
-            }
+            l[j] = route_logit(l[j]);
             lmax = fmaxf(lmax, l[j]);
         }
-        lmax = warp_max(lmax);
-        int* sel = s_sel[warp];
-        float fsum;
-        double sum;
-        const bool sure = route_select<float, NT>(a, l, lmax, reinterpret_cast<float*>(s_keys[warp]), lane, sel, fsum);
-        sum = fsum;
+        lmax = warp_best(lmax);
+
+        float key[NT], sum = 0.f, pmax = 0.f;
+        if (need_p || (!a.sigmoid && !a.renorm)) {
+            if (a.sigmoid) {
+#pragma unroll
+                for (int j = 0; j < NT; j++)  // 0 for -inf
+                    key[j] = __fdividef(1.f, 1.f + __expf(-l[j]));
+            } else {
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    key[j] = l[j] > -INFINITY ? __expf(l[j] - lmax) : 0.f;
+                    sum += key[j];
+                }
+                sum = warp_sum(sum);
+                const float inv = 1.f / sum;
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+                    key[j] *= inv;
+            }
+        }
+        // Two fp32 keys closer than tol may be in the other order in 64 bits.  In half steps, p is off by 5 of its own
+        // for the exponential, 2 |x| for the rounded argument x of it (p |x| is at most pmax max(1, -lmax)), 6 for
+        // reciprocal and product, 20 for a softmax's sum of up to 512 terms in a tree; p + bias by one of the sum's.
+        float tol_p = 0.f;
+        if (need_p) {
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+                pmax = fmaxf(pmax, key[j]);
+            pmax = warp_best(pmax);
+            tol_p = 2.f * 5.97e-8f * ((a.sigmoid ? 12.f : 32.f) + 2.f * fmaxf(1.f, a.sigmoid ? -lmax : 1.f)) * pmax;
+        }
+        constexpr float HALF_STEP2 = 2.f * 5.97e-8f;
+        bool sure = true;
+        Perm perm;
+        float group_best = 0.f, group_next = 0.f;  // of this lane's experts, by what scores groups
+        if (by_logit) {
+            if (need_p) {  // the two best p of the lane are those of its two best logits
+                float b1 = -INFINITY, b2 = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    const float v = l[j] > -INFINITY ? key[j] : -INFINITY;
+                    b2 = v > b1 ? b1 : fmaxf(b2, v);
+                    b1 = fmaxf(b1, v);
+                }
+                group_best = b1;
+                group_next = b2;
+                if (!lanes_of_group) {
+#pragma unroll
+                    for (int j = 0; j < NT; j++)
+                        s_keys[lane * NT + j] = l[j] > -INFINITY ? key[j] : -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+                key[j] = l[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+                key[j] = l[j] > -INFINITY ? key[j] + bias[j] : -INFINITY;
+        }
+        if (a.n_groups > 1 && !lanes_of_group && !(by_logit && need_p)) {
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+                s_keys[lane * NT + j] = key[j];
+        }
+        sort_lane<NT, Perm>(key, perm);
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+            sorted[j][lane] = key[j];
+        __syncwarp();
+
+        if (a.n_groups > 1) {
+            if (!by_logit || !need_p) {
+                group_best = key[0];
+                group_next = NT > 1 ? key[NT > 1 ? 1 : 0] : -INFINITY;
+            }
+            int g = lane;  // the group whose score this lane has
+            if (lanes_of_group) {
+                g = lane / span;
+                for (int o = 1; o < span; o <<= 1) {
+                    const float ob = __shfl_xor_sync(0xffffffffu, group_best, o);
+                    const float on = __shfl_xor_sync(0xffffffffu, group_next, o);
+                    group_next = fmaxf(fminf(group_best, ob), fmaxf(group_next, on));
+                    group_best = fmaxf(group_best, ob);
+                }
+            } else {
+                group_best = group_next = -INFINITY;
+                if (lane < a.n_groups)
+                    for (int i = 0; i < gs; i++) {
+                        const float v = (float)s_keys[lane * gs + i];
+                        group_next = v > group_best ? group_best : fmaxf(group_next, v);
+                        group_best = fmaxf(group_best, v);
+                    }
+            }
+            const float score = g < a.n_groups ? (a.group_top > 1 && group_next > -INFINITY ? group_best + group_next : group_best) : -INFINITY;
+            // a group's place: the groups in front of it
+            int place = 0;
+            const int step = lanes_of_group ? span : 1;
+            for (int i = 0; i < a.n_groups; i++) {
+                const float o = __shfl_sync(0xffffffffu, score, i * step);
+                place += o > score || (o == score && i < g);
+            }
+            const bool in = score > -INFINITY && place < a.topk_groups;
+            if (!(by_logit && a.group_top == 1) && a.topk_groups < a.n_groups) {
+                const float low = -warp_best(in && g < a.n_groups ? -score : -INFINITY);
+                const float high = warp_best(!in && g < a.n_groups ? score : -INFINITY);
+                if (high > -INFINITY)
+                    sure = low - high > 2.f * tol_p + 2.f * HALF_STEP2 * fmaxf(fabsf(low), fabsf(high));
+            }
+            if (lanes_of_group) {
+                if (!in) {
+                    key[0] = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < NT; j++)
+                        sorted[j][lane] = -INFINITY;
+                }
+            } else {
+                const unsigned kept = __ballot_sync(0xffffffffu, in);
+#pragma unroll
+                for (int j = 0; j < NT; j++) {  // in falling order again
+                    const int e = lane * NT + (int)((perm >> (4 * j)) & 15u);
+                    key[j] = e < a.E && ((kept >> (e / gs)) & 1u) ? sorted[j][lane] : -INFINITY;
+                }
+                Perm order = 0;
+                int n = 0;
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+                    if (key[j] > -INFINITY) {
+                        sorted[n][lane] = key[j];
+                        order |= ((perm >> (4 * j)) & 15u) << (4 * n);
+                        n++;
+                    }
+                for (int j = n; j < NT; j++)
+                    sorted[j][lane] = -INFINITY;
+                perm = order;
+                key[0] = sorted[0][lane];
+            }
+        }
+
+        // Rounds: the largest head, of the lowest lane that has it; that lane leaves the expert in `sel` and
+        // moves on.  Lane k keeps the key of round k.
+        float head = key[0], mine_key = -INFINITY;
+        const float* next = &sorted[1][lane];
+        const unsigned lower = (1u << lane) - 1u;
+        auto round = [&](int k) {
+            const float top = warp_best(head);
+            const unsigned has = __ballot_sync(0xffffffffu, head == top);
+            if (lane == k)
+                mine_key = top;
+            if (head == top && top > -INFINITY && !(has & lower)) {  // at most NT times: place NT holds -inf
+                sel[k] = lane * NT + (int)(perm & 15u);
+                head = *next;
+                next += 32;
+                perm >>= 4;
+            }
+            return top;
+        };
+        const int rounds = by_logit ? a.K : a.K + 1;  // the first that is left out has a gap to keep too
+#pragma unroll 1
+        for (int k = 0; k < rounds; k++)
+            round(k);
+        bool close = false;
+        float tol = 0.f;
+        if (!by_logit) {
+            const float before = __shfl_up_sync(0xffffffffu, mine_key, 1);
+            tol = tol_p + HALF_STEP2 * fmaxf(fabsf(before), fabsf(mine_key));
+            close = __any_sync(0xffffffffu, lane > 0 && lane < rounds && mine_key > -INFINITY && !(before - mine_key > tol));
+        }
+        __syncwarp();
+        int mine = lane < a.K && mine_key > -INFINITY ? sel[lane] : -1;
+        if (close && sure) {
+            // Who may be among the K: everybody within tol of the K-th.  A lane each, in 64 bits, then their ranks.
+            const float low = __shfl_sync(0xffffffffu, mine_key, a.K - 1);
+            const float cut = low - (tol_p + HALF_STEP2 * fabsf(low));
+            int n = __popc(__ballot_sync(0xffffffffu, mine_key > -INFINITY));
+            bool more = n == rounds;
+            while (more && n < 32) {
+                const float top = round(n);
+                more = top > -INFINITY && top >= cut;
+                n += more;
+            }
+            __syncwarp();
+            sure = !more;
+            if (sure) {
+                const int e = lane < n ? sel[lane] : 0;
+                double full = 0.0;
+                if (!a.sigmoid) {
+#pragma unroll 1
+                    for (int j = 0; j < NT; j++)
+                    {
+                        const int i = lane * NT + j;
+                        const float v = i < a.E ? route_logit(load_as_float(a.logits, at + i, a.dtype)) : -INFINITY;
+                        if (v > -INFINITY)
+                            full += exp((double)v - (double)lmax);
+                    }
+                    full = warp_sum(full);
+                }
+                double exact = -INFINITY;
+                if (lane < n) {
+                    const double v = route_logit(load_as_float(a.logits, at + e, a.dtype));
+                    exact = (a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - (double)lmax) / full) + (double)fminf(a.bias[e], FLT_MAX);
+                }
+                int rank = 0;
+                for (int i = 0; i < n; i++) {
+                    const double o = __shfl_sync(0xffffffffu, exact, i);
+                    const int oe = __shfl_sync(0xffffffffu, e, i);
+                    rank += o > exact || (o == exact && oe < e);
+                }
+                __syncwarp();
+                if (lane < n)
+                    sel[rank] = e;
+                __syncwarp();
+                mine = lane < a.K && lane < n ? sel[lane] : -1;
+            }
+        }
         if (!sure)
-            route_select<double, NT>(a, l, lmax, s_keys[warp], lane, sel, sum);
-        // weights: lane k has the k-th selected
-        const int e = lane < a.K ? sel[lane] : -1;
-        double w = 0.0;
-        if (e >= 0) {
-            const float v = load_as_float(a.logits, (long long)t * a.stride + e, a.dtype);
-            const double x = fminf(v, FLT_MAX);
-            w = a.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - (double)lmax);
+            mine = route_exact(a, t, lmax, s_keys, lane);
+
+        // The weights, lane k that of slot k.  Where they are divided by their sum, the exponentials are taken
+        // relative to the largest selected, so that weights far below the best expert keep their ratios:
+        // sigmoid(x) = exp(min(x, 0)) / (1 + exp(-|x|)).
+        float w = 0.f;
+        const float x = mine >= 0 ? route_logit(load_as_float(a.logits, at + mine, a.dtype)) : -INFINITY;
+        const float y = a.sigmoid ? fminf(x, 0.f) : x;
+        const float ref = a.renorm ? warp_best(y) : a.sigmoid ? 0.f : lmax;
+        if (mine >= 0) {
+            const float d = y - ref;
+            if (d > -104.f) {  // below, 0 in fp32
+                const float back = (float)(((double)y - (double)ref) - (double)d);  // what rounding d left out
+                w = expf(d);
+                w = fmaf(w, back, w);
+                if (a.sigmoid)
+                    w = w / (1.f + expf(-fabsf(x)));
+            }
         }
         if (a.renorm)
             sum = warp_sum(w);
         if (a.renorm || !a.sigmoid)
-            w = w > 0.0 ? w / sum : 0.0;
+            w = w > 0.f ? w / sum : 0.f;  // sum: of the selected, or of the softmax
         if (lane < a.K) {
-            a.topk_i[(size_t)t * a.K + lane] = e;
-            a.topk_w[(size_t)t * a.K + lane] = (float)(w * (double)a.scale);
-            if (a.counts && e >= 0)
-                atomicAdd(&s_hist[e], 1);
+            a.topk_i[(size_t)t * a.K + lane] = mine;
+            a.topk_w[(size_t)t * a.K + lane] = w * a.scale;
         }
         __syncwarp();
     }
-    if (a.counts) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < a.E; i += blockDim.x)
-            if (s_hist[i])
-                atomicAdd(&a.counts[i], s_hist[i]);
+}
+
+// Slots per expert, from the indices; `counts` were cleared by the kernel in front.
+__global__ void __launch_bounds__(256) route_counts_kernel(const int* __restrict__ topk_i, int n, int E, int* __restrict__ counts) {
+    __shared__ int s_hist[ROUTE_MAX_E];
+    for (int i = threadIdx.x; i < E; i += blockDim.x)
+        s_hist[i] = 0;
+    __syncthreads();
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) {
+        const int e = topk_i[i];
+        if (e >= 0)
+            atomicAdd(&s_hist[e], 1);
     }
+    __syncthreads();
+    for (int i = threadIdx.x; i < E; i += blockDim.x)
+        if (s_hist[i])
+            atomicAdd(&counts[i], s_hist[i]);
 }
 
 }  // namespace op

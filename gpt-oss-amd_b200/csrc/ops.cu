@@ -132,8 +132,9 @@ moe_b200_status moe_b200_route_logits(const void* logits, int dtype, long long s
                                       int topk_groups, int group_top, int renormalize, float scale, int* topk_i,
                                       float* topk_w, int* expert_counts, moe_b200_stream stream) {
     const int E = n_experts, K = experts_per_token;
-    if (n_tokens < 0 || E <= 0 || E > MOE_B200_ROUTE_LOGITS_MAX_EXPERTS)
-        INVALID("moe_b200_route_logits: needs n_tokens >= 0 and n_experts in 1..%d", MOE_B200_ROUTE_LOGITS_MAX_EXPERTS);
+    if (n_tokens < 0 || n_tokens > MOE_B200_ROUTE_LOGITS_MAX_TOKENS || E <= 0 || E > MOE_B200_ROUTE_LOGITS_MAX_EXPERTS)
+        INVALID("moe_b200_route_logits: needs n_tokens in 0..%d and n_experts in 1..%d",
+                MOE_B200_ROUTE_LOGITS_MAX_TOKENS, MOE_B200_ROUTE_LOGITS_MAX_EXPERTS);
     if (K <= 0 || K > MOE_B200_ROUTE_LOGITS_MAX_K || K > E)
         INVALID("moe_b200_route_logits: experts_per_token must be in 1..min(%d, n_experts)", MOE_B200_ROUTE_LOGITS_MAX_K);
     if (!is_float_type(dtype))
@@ -162,21 +163,32 @@ moe_b200_status moe_b200_route_logits(const void* logits, int dtype, long long s
     if (moe_b200_status st = current_device(&dev, &sms))
         return st;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (expert_counts) {
-        cudaError_t e = cudaMemsetAsync(expert_counts, 0, sizeof(int) * (size_t)E, st);
-        if (e != cudaSuccess)
-            return launched("moe_b200_route_logits: counts", e);
-        if (n_tokens == 0)
-            return MOE_B200_OK;
-    }
+    if (n_tokens == 0)
+        return launched("moe_b200_route_logits: counts", cudaMemsetAsync(expert_counts, 0, sizeof(int) * (size_t)E, st));
     LogitsArgs a{logits, stride, dtype, n_tokens, E, K, score == MOE_B200_SCORE_SIGMOID, bias, n_groups, topk_groups,
                  group_top, renormalize != 0, scale, topk_i, topk_w, expert_counts};
-    const int warps = n_tokens >= ROUTE_WARPS * sms ? ROUTE_WARPS : 1;
-    const int want = (n_tokens + warps - 1) / warps, most = 32 * sms;
-    const int grid = want < most ? want : most;
-    auto kernel = E <= 32 ? route_logits_kernel<1> : E <= 64 ? route_logits_kernel<2> : E <= 128 ? route_logits_kernel<4>
-                  : E <= 256 ? route_logits_kernel<8> : route_logits_kernel<16>;
-    kernel<<<grid, 32 * warps, 0, st>>>(a);
+    // a warp per token; small batches spread over the SMs
+    const int warps = n_tokens >= 2 * ROUTE_WARPS * sms ? ROUTE_WARPS : n_tokens >= 4 * sms ? 4 : 1;
+    const int want = (n_tokens + warps - 1) / warps, most = 2 * (ROUTE_WARPS / warps) * sms;
+    const int nt = E <= 32 ? 1 : E <= 64 ? 2 : E <= 128 ? 4 : E <= 256 ? 8 : 16;
+    const int piece = nt * size_of(dtype) < 16 ? nt * size_of(dtype) : 16;
+    const bool vec = E % nt == 0 && rows_aligned(logits, stride, size_of(dtype), piece);
+    auto kernel = nt == 1 ? (vec ? route_logits_kernel<1, true> : route_logits_kernel<1, false>)
+                  : nt == 2 ? (vec ? route_logits_kernel<2, true> : route_logits_kernel<2, false>)
+                  : nt == 4 ? (vec ? route_logits_kernel<4, true> : route_logits_kernel<4, false>)
+                  : nt == 8 ? (vec ? route_logits_kernel<8, true> : route_logits_kernel<8, false>)
+                            : (vec ? route_logits_kernel<16, true> : route_logits_kernel<16, false>);
+    const size_t smem = sizeof(double) * 32 * nt * warps;
+    if (nt >= 8 && smem > 16 * 1024) {  // with the fixed part more than a block has without asking
+        cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024);
+        if (e != cudaSuccess)
+            return launched("moe_b200_route_logits: shared memory", e);
+    }
+    kernel<<<want < most ? want : most, 32 * warps, smem, st>>>(a);
+    if (expert_counts) {
+        const int n = n_tokens * K, blocks = (n + 2047) / 2048;
+        route_counts_kernel<<<blocks < sms ? blocks : sms, 256, 0, st>>>(topk_i, n, E, expert_counts);
+    }
     return launched("moe_b200_route_logits", cudaGetLastError());
 }
 

@@ -447,6 +447,7 @@ moe_b200_status moe_b200_add_rmsnorm(const void* x, int x_dtype, long long x_str
  * expert, overwritten. */
 #define MOE_B200_SCORE_SOFTMAX 0
 #define MOE_B200_SCORE_SIGMOID 1
+#define MOE_B200_ROUTE_LOGITS_MAX_TOKENS 16777216
 #define MOE_B200_ROUTE_LOGITS_MAX_EXPERTS 512
 #define MOE_B200_ROUTE_LOGITS_MAX_K 16
 moe_b200_status moe_b200_route_logits(const void* logits, int dtype, long long stride, int n_tokens, int n_experts,

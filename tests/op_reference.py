@@ -39,8 +39,10 @@ def route(logits, k, score, bias, n_groups, topk_groups, group_top, renorm, scal
         if score == "softmax":
             z = sum(math.exp(v - m) for v in l.values())
             p = {e: math.exp(v - m) / z for e, v in l.items()}
+            logp = {e: v - m - math.log(z) for e, v in l.items()}
         else:
             p = {e: 1 / (1 + math.exp(-v)) if v > -700 else 0.0 for e, v in l.items()}
+            logp = {e: -math.log1p(math.exp(-v)) if v > -700 else v for e, v in l.items()}
         key = {e: l[e] if B is None else p[e] + min(float(B[e]), fmax) for e in live}
         if n_groups > 1:
             size = E // n_groups
@@ -53,10 +55,12 @@ def route(logits, k, score, bias, n_groups, topk_groups, group_top, renorm, scal
             kept = {g for _, g in sorted(scores)[:topk_groups]}
             key = {e: v for e, v in key.items() if e // size in kept}
         chosen = sorted(key, key=lambda e: (-key[e], e))[:k]
-        total = sum(p[e] for e in chosen)
+        # p / sum of the selected p; relative to the largest of them, which 64 bits hold whatever the logits
+        big = max((logp[e] for e in chosen), default=0.0)
+        total = sum(math.exp(logp[e] - big) for e in chosen)
         for j, e in enumerate(chosen):
             idx[t, j] = e
-            w[t, j] = (p[e] / total if total > 0 else 0.0) * scale if renorm else p[e] * scale
+            w[t, j] = (math.exp(logp[e] - big) / total if renorm else p[e]) * scale
     return idx, w
 
 

@@ -153,15 +153,18 @@ def test_add_rmsnorm_mx_scale_on_the_border():
 # -- route_logits ---------------------------------------------------------------
 
 
+# Relative error of a weight before its last rounding, in steps of fp32 (2^-23): two exponentials of 2 each, 1 + e,
+# the division by it; the sum it is divided by: terms off by 6 each, up to 9 + 4 roundings of half a step in it (a
+# softmax over 512 experts: 16 in a lane, 5 levels; its exponentials' arguments are rounded: 0.37); the division, the scale.
+WEIGHT_ERROR = (6 + 6 + 11 + 0.37 + 1) * 2.0**-23
+
+
 def _check_route(logits, k, r, **kw):
     a = dict(score="softmax", bias=None, n_groups=1, topk_groups=1, group_top=2, renormalize=True, scale=1.0)
     a.update(kw)
     idx, w = ref.route(logits, k, a["score"], a["bias"], a["n_groups"], a["topk_groups"], a["group_top"], a["renormalize"], a["scale"])
     assert torch.equal(r.topk_i.cpu(), idx)
-    # 64-bit exponentials, an fp32 sum of a softmax that is not renormalised: its exponentials are off by
-    # at most 2 steps and a rounded difference (x e^-x <= 0.37), the sum by 9 + 4 roundings
-    err = w.abs() * (2 + 0.37 + 13) * 2.0**-23
-    _close(r.topk_w.cpu(), w, err, F32, "weights")
+    _close(r.topk_w.cpu(), w, w.abs() * WEIGHT_ERROR, F32, "weights")
     if r.counts is not None:
         flat = idx[idx >= 0].long()
         assert torch.equal(r.counts.cpu().long(), torch.bincount(flat, minlength=logits.shape[1]))
@@ -265,10 +268,26 @@ def test_route_logits_large_batch_strides_and_rows_behind():
     key, idx = (p + bias.double()).sort(dim=1, descending=True, stable=True)
     assert torch.equal(r.topk_i.long(), idx[:, :k])
     w = p.gather(1, idx[:, :k])
-    _close(r.topk_w, w / w.sum(1, keepdim=True) * 2, w * 2.0**-45, F32)  # 64-bit exponentials
+    w = w / w.sum(1, keepdim=True) * 2
+    _close(r.topk_w, w, w * WEIGHT_ERROR, F32)
     pick = torch.arange(0, T, 1999, device="cuda")
     s = pkg.route_logits(logits[pick].contiguous(), k, **kw)
     assert torch.equal(s.topk_i, r.topk_i[pick]) and torch.equal(s.topk_w, r.topk_w[pick])
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_logits_weights_far_below_the_best_expert(score):
+    """A bias chooses experts whose scores are below fp32's range beside the best one: the ratios of their
+    weights stay."""
+    E, k = 40, 4
+    logits = torch.full((2, E), -130.0, device="cuda")
+    logits[:, 0] = 60.0
+    logits[0, 5:9] = torch.tensor([-100.0, -101.0, -102.5, -130.0], device="cuda")
+    logits[1, 5:9] = torch.tensor([-300.0, -301.0, -302.5, -300.25], device="cuda")
+    bias = torch.zeros(E, device="cuda")
+    bias[5:9] = torch.tensor([5.0, 4.0, 3.0, 2.0], device="cuda")
+    kw = dict(score=score, bias=bias)
+    _check_route(logits, k, pkg.route_logits(logits, k, **kw), **kw)
 
 
 def test_route_logits_agrees_with_the_block():

@@ -46,7 +46,7 @@ def test_add_rmsnorm_refuses(kw):
 
 
 @pytest.mark.parametrize("kw", [
-    dict(T=-1), dict(E=0), dict(E=513), dict(K=0), dict(K=17), dict(E=3, K=4), dict(dt=3), dict(score=2), dict(ng=0), dict(ng=3),
+    dict(T=-1), dict(T=16777217), dict(E=0), dict(E=513), dict(K=0), dict(K=17), dict(E=3, K=4), dict(dt=3), dict(score=2), dict(ng=0), dict(ng=3),
     dict(E=66, ng=33), dict(ng=4, kg=0), dict(ng=4, kg=5), dict(ng=4, kg=1, gt=0), dict(ng=4, kg=1, gt=3), dict(ng=32, kg=1, gt=1),
     dict(E=32, ng=32, kg=8, gt=2), dict(scale=float("nan")), dict(scale=float("inf")), dict(l=None), dict(i=None), dict(w=None),
     dict(s=-1), dict(l=A + 2), dict(bias=A + 1), dict(i=A + 1), dict(w=A + 2), dict(c=A + 3)])
