@@ -6,7 +6,7 @@
 // for a bf16 x, an fp32 residual, a bf16 y and codes.  For many rows HBM bounds it, for one row
 // the chain load -> sum over the block -> store.
 //
-// A block owns a row and a thread 8 * NV columns of it in registers.  VEC: eight neighbouring
+// A block owns a row (a warp, where a warp holds it and there are many) and a thread 8 * NV columns of it in registers.  VEC: eight neighbouring
 // columns per step, moved 16 bytes at a time (rows on 16-byte boundaries, H a multiple of 8).
 // Otherwise a warp covers the same 256 columns with eight coalesced steps of one element per lane.
 //
@@ -29,7 +29,7 @@ struct NormArgs {
     const void* w;
     int w_dtype;
     float eps;
-    int H;
+    int n_rows, H;
     void* y;  // null: none
     long long y_stride;
     int y_dtype;
@@ -38,6 +38,7 @@ struct NormArgs {
     void* scales;   // [rows, n_scales], f32 or e8m0
     int n_scales;
     int group;      // columns per scale: 32, 64, 128; 0: the row
+    int group_shift;
     int mx;         // e8m0 scales
 };
 
@@ -178,7 +179,9 @@ __device__ __forceinline__ float norm_put_scale(const NormArgs& a, long long i, 
 template <bool VEC, int NV>
 __global__ void __launch_bounds__(1024) add_rmsnorm_kernel(const NormArgs a) {
     __shared__ float slots[64];
-    const long long row = blockIdx.x;
+    const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;  // blockDim.y > 1: a warp per row
+    if (row >= a.n_rows)
+        return;
     const int H = a.H;
     const int lane = threadIdx.x & 31;
     float r[NV][8];
@@ -245,7 +248,7 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_kernel(const NormArgs a) {
                     m = fmaxf(m, fabsf(r[v][e]));
                 for (int o = 1; o < a.group / 8; o <<= 1)
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                inv = norm_put_scale(a, s0 + c / a.group, m, c < H && c % a.group == 0);
+                inv = norm_put_scale(a, s0 + (c >> a.group_shift), m, c < H && (c & (a.group - 1)) == 0);
             }
             if (c < H) {
                 uint2 d;
@@ -254,24 +257,39 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_kernel(const NormArgs a) {
                 *reinterpret_cast<uint2*>(q + c) = d;
             }
         } else {
+            // a group is one, two or four steps of a warp
             float inv[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++)  // non-negative floats order like their bits
-                inv[e] = a.group ? __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(r[v][e]), 0.f))))
-                                 : inv_row;
-            if (a.group >= 64)
+            for (int e = 0; e < 8; e++)
+                inv[e] = inv_row;
+            if (a.group) {
+                float m[8];
 #pragma unroll
-                for (int e = 0; e < 8; e += 2)
-                    inv[e] = inv[e + 1] = fmaxf(inv[e], inv[e + 1]);
-            if (a.group >= 128)
+                for (int e = 0; e < 8; e++)  // non-negative floats order like their bits; NaN counts as 0
+                    m[e] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(r[v][e]), 0.f))));
+                const int c0 = norm_col<false>(v, 0) - lane;
+                auto scale_of = [&](int e, float top) {
+                    const int c = c0 + e * 32;
+                    return norm_put_scale(a, s0 + (c >> a.group_shift), top, lane == 0 && c < H);
+                };
+                if (a.group == 32) {
 #pragma unroll
-                for (int e = 0; e < 8; e += 4)
-                    inv[e] = inv[e + 1] = inv[e + 2] = inv[e + 3] = fmaxf(inv[e], inv[e + 2]);
+                    for (int e = 0; e < 8; e++)
+                        inv[e] = scale_of(e, m[e]);
+                } else if (a.group == 64) {
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2)
+                        inv[e] = inv[e + 1] = scale_of(e, fmaxf(m[e], m[e + 1]));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e += 4)
+                        inv[e] = inv[e + 1] = inv[e + 2] = inv[e + 3] =
+                            scale_of(e, fmaxf(fmaxf(m[e], m[e + 1]), fmaxf(m[e + 2], m[e + 3])));
+                }
+            }
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const int c = norm_col<false>(v, e);
-                if (a.group)
-                    inv[e] = norm_put_scale(a, s0 + c / a.group, inv[e], lane == 0 && c < H && c % a.group == 0);
                 if (c < H)
                     q[c] = (uint8_t)(floats_to_e4m3x2(r[v][e] * inv[e], 0.f) & 0xFFu);
             }

@@ -111,8 +111,8 @@ moe_b200_status moe_b200_add_rmsnorm(const void* x, int x_dtype, long long x_str
     if (moe_b200_status st = current_device(&dev, &sms))
         return st;
     NormArgs a{x, x_stride, x_dtype, residual, residual_out, residual_stride, residual_out_stride, residual_dtype,
-               weight, weight_dtype, eps, H, y, y_stride, y_dtype, static_cast<uint8_t*>(q), q_stride, q_scales,
-               n_scales, group, mx};
+               weight, weight_dtype, eps, n_rows, H, y, y_stride, y_dtype, static_cast<uint8_t*>(q), q_stride, q_scales,
+               n_scales, group, group == 128 ? 7 : group == 64 ? 6 : 5, mx};
     const bool vec = H % 8 == 0 && rows_aligned(x, x_stride, size_of(x_dtype), 16) && aligned(weight, 16) &&
                      (!residual || rows_aligned(residual, residual_stride, size_of(residual_dtype), 16)) &&
                      (!residual_out || rows_aligned(residual_out, residual_out_stride, size_of(residual_dtype), 16)) &&
@@ -123,7 +123,8 @@ moe_b200_status moe_b200_add_rmsnorm(const void* x, int x_dtype, long long x_str
     const int threads = 32 * ((chunks + nv - 1) / nv);
     auto kernel = vec ? (nv == 1 ? add_rmsnorm_kernel<true, 1> : nv == 2 ? add_rmsnorm_kernel<true, 2> : add_rmsnorm_kernel<true, 4>)
                       : (nv == 1 ? add_rmsnorm_kernel<false, 1> : nv == 2 ? add_rmsnorm_kernel<false, 2> : add_rmsnorm_kernel<false, 4>);
-    kernel<<<n_rows, threads, 0, st>>>(a);
+    const int together = threads == 32 && n_rows >= 8 * sms ? 8 : 1;  // rows per block
+    kernel<<<(n_rows + together - 1) / together, dim3(threads, together), 0, st>>>(a);
     return launched("moe_b200_add_rmsnorm", cudaGetLastError());
 }
 

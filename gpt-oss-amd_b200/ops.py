@@ -19,6 +19,8 @@ _FLOATS = {torch.float32: capi.DTYPE_F32, torch.bfloat16: capi.DTYPE_BF16, torch
 _X4 = {torch.bfloat16: capi.DTYPE_BF16, torch.float16: capi.DTYPE_F16, torch.float8_e4m3fn: capi.DTYPE_E4M3}
 _QUANT = {"row": capi.SCALE_ROW, 32: capi.SCALE_G32, 64: capi.SCALE_G64, 128: capi.SCALE_G128, "mx": capi.SCALE_MX}
 _MX_TYPES = (torch.float8_e8m0fnu, torch.uint8)
+_F32, _I32, _U8, _E4M3 = (torch.float32,), (torch.int32,), (torch.uint8,), (torch.float8_e4m3fn,)
+_W4_SCALES, _X_SCALES = (torch.bfloat16, *_MX_TYPES), (torch.float32, *_MX_TYPES)
 
 
 class NormResult(NamedTuple):
@@ -39,32 +41,48 @@ def _need(ok, text):
         raise ValueError(text)
 
 
-def _rows(t, name, shape, types, device):
+# These run in front of kernels of a few microseconds: a tensor's shape, strides and device are asked for once each.
+
+
+def _wrong(t, name, shape, types, dev, what):
+    raise ValueError(f"{name}: needs {what} {tuple(shape)} on cuda:{dev}, one of {[str(d) for d in types]}; "
+                     f"got {tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
+
+
+def _rows(t, name, rows, cols, types, dev):
     """Checks a 2-d tensor with neighbouring columns; returns its address and row stride."""
-    if t.dtype not in types or t.shape != shape or t.device != device or (t.stride(1) != 1 and shape[1] > 1):
-        raise ValueError(f"{name}: needs {tuple(shape)} on {device} with contiguous rows, one of "
-                         f"{[str(d) for d in types]}; got {tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
-    return t.data_ptr(), t.stride(0)
+    if t.dtype not in types or t.get_device() != dev or t.shape != (rows, cols):
+        _wrong(t, name, (rows, cols), types, dev, "contiguous rows of")
+    stride, one = t.stride()
+    if one != 1 and cols > 1:
+        _wrong(t, name, (rows, cols), types, dev, "contiguous rows of")
+    return t.data_ptr(), stride
 
 
-def _dense(t, name, shape, types, device):
-    if t.dtype not in types or t.shape != shape or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name}: needs contiguous {tuple(shape)} on {device}, one of {[str(d) for d in types]}; "
-                         f"got {tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
+def _dense(t, name, shape, types, dev):
+    if t.dtype not in types or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
+        _wrong(t, name, shape, types, dev, "contiguous")
     return t.data_ptr()
 
 
-def _call(fn, device, stream, *args):
-    L = capi.lib()
-    _need(device.type == "cuda", "needs CUDA tensors: there is no CPU path")
-    s = (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream
-    if device.index == torch.cuda.current_device():
-        status = getattr(L, fn)(*args, s)
+def _device(t):
+    """The CUDA device index of the first tensor of a call."""
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError("needs CUDA tensors: there is no CPU path")
+    return dev
+
+
+def _call(name, dev, stream, *args):
+    fn = getattr(capi.lib(), name)
+    raw = torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
+    if dev == torch._C._cuda_getDevice():
+        status = fn(*args, raw)
     else:
-        with torch.cuda.device(device):
-            status = getattr(L, fn)(*args, s)
+        with torch.cuda.device(dev):
+            status = fn(*args, raw)
     if status:
-        capi.check(status, None, L)
+        capi.check(status)
 
 
 def add_rmsnorm(x, weight, residual=None, *, eps=1e-5, dtype=torch.bfloat16, quant=None, residual_out=None, out=None,
@@ -76,40 +94,40 @@ def add_rmsnorm(x, weight, residual=None, *, eps=1e-5, dtype=torch.bfloat16, qua
     be ``residual`` itself), in residual's type.  ``quant``: "row", 32, 64 or 128 (fp32 scales per row or
     group of columns) or "mx" (e8m0 per 32): q is float8_e4m3fn [T, H], q_scales [T, scales per row]
     float32, with "mx" float8_e8m0fnu (uint8 is taken too)."""
+    dev = _device(x)
     _need(x.dim() == 2, "x: needs two dimensions")
-    T, H = shape = x.shape
-    dev = x.device
-    xp, xs = _rows(x, "x", shape, _FLOATS, dev)
+    T, H = x.shape
+    xp, xs = _rows(x, "x", T, H, _FLOATS, dev)
     wp = _dense(weight, "weight", (H,), _FLOATS, dev)
-    rp = rs = rop = ros = yp = ys = qp = qs = sp = None
-    rt = yt = kind = 0
+    rp = rop = yp = qp = sp = None
+    rt = rs = ros = yt = ys = qs = kind = 0
     if residual is not None:
-        rp, rs = _rows(residual, "residual", shape, _FLOATS, dev)
+        rp, rs = _rows(residual, "residual", T, H, _FLOATS, dev)
         rt = _FLOATS[residual.dtype]
         if residual_out is None:
-            residual_out = torch.empty(shape, dtype=residual.dtype, device=dev)
-        rop, ros = _rows(residual_out, "residual_out", shape, (residual.dtype,), dev)
-    else:
-        _need(residual_out is None, "residual_out without residual")
+            residual_out = torch.empty(T, H, dtype=residual.dtype, device=x.device)
+        rop, ros = _rows(residual_out, "residual_out", T, H, (residual.dtype,), dev)
+    elif residual_out is not None:
+        raise ValueError("residual_out without residual")
     if out is not None or dtype is not None:
         if out is None:
-            out = torch.empty(shape, dtype=dtype, device=dev)
-        yp, ys = _rows(out, "out", shape, _FLOATS, dev)
+            out = torch.empty(T, H, dtype=dtype, device=x.device)
+        yp, ys = _rows(out, "out", T, H, _FLOATS, dev)
         yt = _FLOATS[out.dtype]
     if quant is not None:
         _need(quant in _QUANT, f"quant: one of {list(_QUANT)}")
         kind = _QUANT[quant]
         n = 1 if quant == "row" else -(-H // (32 if quant == "mx" else quant))
         if q is None:
-            q = torch.empty(shape, dtype=torch.float8_e4m3fn, device=dev)
+            q = torch.empty(T, H, dtype=torch.float8_e4m3fn, device=x.device)
         if q_scales is None:
-            q_scales = torch.empty(T, n, dtype=torch.float8_e8m0fnu if quant == "mx" else torch.float32, device=dev)
-        qp, qs = _rows(q, "q", shape, (torch.float8_e4m3fn,), dev)
-        sp = _dense(q_scales, "q_scales", (T, n), _MX_TYPES if quant == "mx" else (torch.float32,), dev)
-    else:
-        _need(q is None and q_scales is None, "q without quant")
-    _call("moe_b200_add_rmsnorm", dev, stream, xp, _FLOATS[x.dtype], xs, rp, rt, rs or 0, rop, ros or 0, wp,
-          _FLOATS[weight.dtype], eps, T, H, yp, yt, ys or 0, qp, qs or 0, sp, kind)
+            q_scales = torch.empty(T, n, dtype=torch.float8_e8m0fnu if quant == "mx" else torch.float32, device=x.device)
+        qp, qs = _rows(q, "q", T, H, _E4M3, dev)
+        sp = _dense(q_scales, "q_scales", (T, n), _MX_TYPES if quant == "mx" else _F32, dev)
+    elif q is not None or q_scales is not None:
+        raise ValueError("q without quant")
+    _call("moe_b200_add_rmsnorm", dev, stream, xp, _FLOATS[x.dtype], xs, rp, rt, rs, rop, ros, wp, _FLOATS[weight.dtype], eps,
+          T, H, yp, yt, ys, qp, qs, sp, kind)
     return NormResult(out, residual_out, q, q_scales)
 
 
@@ -127,25 +145,25 @@ def route_logits(logits, k, *, score="softmax", bias=None, n_groups=1, topk_grou
     ``scale`` multiplies them.  Ties go to the lower index.  Experts with a logit of -inf or NaN take no
     part; empty slots have index -1 and weight 0.  ``counts``: True or an int32 [E] tensor for the number
     of slots per expert.  ``topk_i``, ``topk_w``: where the results go."""
+    dev = _device(logits)
     _need(logits.dim() == 2, "logits: needs two dimensions")
-    T, E = shape = logits.shape
-    dev = logits.device
-    lp, ls = _rows(logits, "logits", shape, _FLOATS, dev)
+    T, E = logits.shape
+    lp, ls = _rows(logits, "logits", T, E, _FLOATS, dev)
     _need(score in _SCORES, f"score: one of {list(_SCORES)}")
-    bp = None if bias is None else _dense(bias, "bias", (E,), (torch.float32,), dev)
+    bp = None if bias is None else _dense(bias, "bias", (E,), _F32, dev)
     if topk_i is None:
-        topk_i = torch.empty(T, k, dtype=torch.int32, device=dev)
+        topk_i = torch.empty(T, k, dtype=torch.int32, device=logits.device)
     if topk_w is None:
-        topk_w = torch.empty(T, k, dtype=torch.float32, device=dev)
-    ip = _dense(topk_i, "topk_i", (T, k), (torch.int32,), dev)
-    wp = _dense(topk_w, "topk_w", (T, k), (torch.float32,), dev)
+        topk_w = torch.empty(T, k, dtype=torch.float32, device=logits.device)
+    ip = _dense(topk_i, "topk_i", (T, k), _I32, dev)
+    wp = _dense(topk_w, "topk_w", (T, k), _F32, dev)
     cp = None
     if counts is True:
-        counts = torch.empty(E, dtype=torch.int32, device=dev)
+        counts = torch.empty(E, dtype=torch.int32, device=logits.device)
     elif counts is False:
         counts = None
     if counts is not None:
-        cp = _dense(counts, "counts", (E,), (torch.int32,), dev)
+        cp = _dense(counts, "counts", (E,), _I32, dev)
     _call("moe_b200_route_logits", dev, stream, lp, _FLOATS[logits.dtype], ls, T, E, k, _SCORES[score], bp, n_groups,
           topk_groups, group_top, bool(renormalize), scale, ip, wp, cp)
     return Routing(topk_i, topk_w, counts)
@@ -162,31 +180,27 @@ def w4_matvec(x, codes, scales, bias=None, *, x_scales=None, ids=None, rows_per_
     int32 [M], one matrix per row of the result, an index outside the stack gives zeros; without
     it M = x rows * rows_per_x.  ``swiglu``: (alpha, limit) for the framework's clamped SwiGLU over
     interleaved gate and up rows.  At most 256 rows."""
+    dev = _device(x)
     _need(x.dim() == 2, "x: needs two dimensions")
     rows, K = x.shape
-    dev = x.device
-    xp, xs = _rows(x, "x", x.shape, _X4, dev)
-    stack = scales.dim() == 3
-    _need(scales.dim() in (2, 3), "scales: needs [N, groups] or [n, N, groups]")
-    n = scales.shape[0] if stack else 1
-    N, G = scales.shape[-2:]
-    lead = (n, N) if stack else (N,)
+    xp, xs = _rows(x, "x", rows, K, _X4, dev)
+    shape = scales.shape
+    stack = len(shape) == 3
+    _need(stack or len(shape) == 2, "scales: needs [N, groups] or [n, N, groups]")
+    N, G = shape[-2], shape[-1]
+    lead = shape[:-1]
     _need(G > 0 and K % G == 0, "scales: their number must divide the columns of x")
-    group = K // G
-    if codes.dim() == len(lead) + 2:
-        cp = _dense(codes, "codes", (*lead, G, 16), (torch.uint8,), dev)
-    else:
-        cp = _dense(codes, "codes", (*lead, K // 2), (torch.uint8,), dev)
-    fmt = capi.W4_INT4 if scales.dtype == torch.bfloat16 else capi.W4_MXFP4
-    sp = _dense(scales, "scales", (*lead, G), (torch.bfloat16, *_MX_TYPES), dev)
-    bp = None if bias is None else _dense(bias, "bias", lead, (torch.float32,), dev)
+    cp = _dense(codes, "codes", (*lead, G, 16) if codes.dim() == len(shape) + 1 else (*lead, K // 2), _U8, dev)
+    sp = _dense(scales, "scales", shape, _W4_SCALES, dev)
+    bp = None if bias is None else _dense(bias, "bias", lead, _F32, dev)
     _need(rows_per_x >= 1, "rows_per_x: at least 1")
     M = rows * rows_per_x
     ip = None
     if ids is not None:
-        _need(M - rows_per_x < ids.numel() <= M, "ids: one per row, rows_per_x for each row of x")
-        M = ids.numel()
-        ip = _dense(ids, "ids", (M,), (torch.int32,), dev)
+        n = ids.numel()
+        _need(M - rows_per_x < n <= M, "ids: one per row, rows_per_x for each row of x")
+        M = n
+        ip = _dense(ids, "ids", (M,), _I32, dev)
     else:
         _need(not stack, "a stack of matrices needs ids")
     kind, xsp = capi.SCALE_NONE, None
@@ -201,13 +215,14 @@ def w4_matvec(x, codes, scales, bias=None, *, x_scales=None, ids=None, rows_per_
             fits = [s for s in (32, 64, 128) if -(-K // s) == m]
             _need(len(fits) == 1, "x_scales: one per row or per 32, 64 or 128 columns")
             kind, want = _QUANT[fits[0]], m
-        xsp = _dense(x_scales, "x_scales", (rows, want), (torch.float32, *_MX_TYPES), dev)
+        xsp = _dense(x_scales, "x_scales", (rows, want), _X_SCALES, dev)
     alpha, limit = swiglu if swiglu is not None else (0.0, 0.0)
     n_out = N if swiglu is None else N // 2
     if out is None:
-        out = torch.empty(M, n_out, dtype=dtype, device=dev)
-    op, os_ = _rows(out, "out", (M, n_out), _FLOATS, dev)
-    w = capi.W4Matrix(fmt, group, n, N, K, cp, sp, bp)
+        out = torch.empty(M, n_out, dtype=dtype, device=x.device)
+    op, os_ = _rows(out, "out", M, n_out, _FLOATS, dev)
+    w = capi.W4Matrix(capi.W4_INT4 if scales.dtype == torch.bfloat16 else capi.W4_MXFP4, K // G, shape[0] if stack else 1, N, K,
+                      cp, sp, bp)
     _call("moe_b200_w4_matvec", dev, stream, ctypes.byref(w), xp, _X4[x.dtype], xs, xsp, kind, M, rows_per_x, ip,
           swiglu is not None, alpha, limit, op, _FLOATS[out.dtype], os_)
     return out

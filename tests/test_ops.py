@@ -68,7 +68,7 @@ def _check_norm(x, w, res, r, quant, eps=1e-5):
     (2, 1, F32, F32, F32, "row"), (4, 31, BF16, None, None, "mx"), (7, 33, F32, BF16, BF16, 32), (6, 200, F16, F16, None, 128),
     (33, 2047, F16, F32, BF16, 128), (300, 2880, F32, F32, BF16, "mx"), (1000, 2888, BF16, F32, None, 64), (700, 4096, BF16, BF16, BF16, "row"),
     (2, 8192, BF16, F32, BF16, 128), (400, 8200, F32, None, F32, 64), (2, 16392, BF16, F32, F16, "row"), (3, 32768, F32, F32, BF16, "mx"),
-    (2, 32767, BF16, F16, F32, 128), (2, 9999, F32, F32, BF16, "row")])
+    (2, 32767, BF16, F16, F32, 128), (2, 9999, F32, F32, BF16, "row"), (3001, 64, BF16, F32, BF16, "row"), (1203, 255, F16, F16, F32, 64)])
 def test_add_rmsnorm(T, H, xt, rt, yt, quant):
     g = _gen(T * 40009 + H)
     x = (3 * _randn(g, T, H)).to(xt)
