@@ -16,7 +16,7 @@ using namespace moe::op;
 namespace {
 
 constexpr int MAX_DEVICES = 64;
-constexpr size_t MV_MAX_SMEM = 212 * 1024;  // dynamic shared memory of w4_matvec_kernel
+constexpr size_t MV_SM_SMEM = 228 * 1024;  // of an SM
 
 moe_b200_status refuse(moe_b200_status st, const char* fmt, ...) {
     va_list ap;
@@ -273,38 +273,64 @@ moe_b200_status moe_b200_w4_matvec(const moe_b200_w4_matrix* w, const void* x, i
     a.out_stride = out_stride;
     a.out_dtype = out_dtype;
     a.n_tiles = (N + MV_TILE - 1) / MV_TILE;
-    a.ksplit = a.n_tiles < 1024 ? 4 : 2;  // by the matrix alone: a row's sums have one order in every batch
-    while (a.ksplit > (mv_steps(K) + 1) / 2)
-        a.ksplit /= 2;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
 
     // Pairs of x rows per pass over the weights.  Chosen matrices are shared by n_rows / n_mats rows on the average.
     const int share = ids ? (n_rows + w->n_mats - 1) / w->n_mats : n_rows;
-    int pairs = share <= 2 ? 1 : share <= 4 ? 2 : 4;
-    auto smem_of = [&](int p) { return mv_smem_bytes(K, p, n_rows < 2 * p ? n_rows : 2 * p); };
-    while (pairs > 1 && smem_of(pairs) > MV_MAX_SMEM)
-        pairs /= 2;
-    const size_t smem = smem_of(pairs);
-    const long long scale_bytes = (long long)w->n_mats * N * (K / w->group) * (int4 ? 2 : 1);
-    const bool words = !(int4 && w->group == 32 && (K / 32) % 2) && aligned(w->scales, 4) && scale_bytes % 4 == 0;
-    const int sh = words ? a.group_shift : MV_DIRECT;
+    int pairs = share <= 2 ? 1 : 2;
+    const int steps = mv_steps(K), sb = int4 ? 2 : 1, SG = (K / 32) >> a.group_shift;
+    a.scale_slot = (MV_TILE * SG * sb + 15) / 16 * 16;
+    a.scale_bulk = ((reinterpret_cast<uintptr_t>(w->scales) | (ids ? (unsigned long long)N * SG * sb : 0)) & 15) == 0;
+    // The ring: two blocks per SM where two stages of whole rows fit, else pieces of rows, else one block.
+    size_t smem = 0;
+    int blocks = 0;
+    for (;; pairs /= 2) {
+        const size_t fixed = 1024 + mv_static_bytes(pairs);  // the system's and the kernel's own
+        const size_t x_bytes = 128 + (size_t)(n_rows < 2 * pairs ? n_rows : 2 * pairs) * steps * 272;
+        for (blocks = 2; blocks >= 1 && !smem; blocks--) {
+            const size_t room = MV_SM_SMEM / blocks - fixed;
+            const int pieces[5] = {steps, 32, 24, 16, 8};  // steps of a stage: a row, or multiples of the eight warps
+            for (int i = steps <= 48 ? 0 : 1; i < 5 && !smem; i++) {
+                const int cs = pieces[i];
+                if (i > 0 && cs >= steps)
+                    continue;
+                const int pitch = cs == steps ? K / 2 : cs * 64 + 64;  // pieces of rows 64 modulo 128 apart
+                const int nc = (steps + cs - 1) / cs;
+                for (int d = MV_MAX_DEPTH; d >= 3 && !smem; d--) {
+                    const int slots = (d - 1 + nc - 1) / nc + 1;  // tiles begun or ahead
+                    const size_t need = (size_t)d * MV_TILE * pitch + (size_t)slots * a.scale_slot + x_bytes;
+                    if (need <= room) {
+                        a.depth = d;
+                        a.chunk_steps = cs;
+                        a.pitch = pitch;
+                        a.scale_slots = slots;
+                        smem = need;
+                    }
+                }
+            }
+        }
+        blocks++;
+        if (smem || pairs == 1)
+            break;
+    }
+    if (!smem)
+        INVALID("moe_b200_w4_matvec: rows too long for shared memory");
+    a.row_map = a.pitch % 64 == 32 ? 1 : a.pitch % 32 == 16 ? 2 : 0;
+    const bool paired = a.group_shift == 0 && (K / 32) % 2 == 0;
     typedef void (*Kernel)(MatvecArgs);
-#define MV_ROW(I4, S) {w4_matvec_kernel<I4, S, 1>, w4_matvec_kernel<I4, S, 2>, w4_matvec_kernel<I4, S, 4>}
-    static const Kernel kernels[2][4][3] = {
-        {MV_ROW(false, 0), {nullptr, nullptr, nullptr}, {nullptr, nullptr, nullptr}, MV_ROW(false, MV_DIRECT)},
-        {MV_ROW(true, 0), MV_ROW(true, 1), MV_ROW(true, 2), MV_ROW(true, MV_DIRECT)}};
+#define MV_ROW(I4, PR) {w4_matvec_kernel<I4, PR, 1>, w4_matvec_kernel<I4, PR, 2>}
+    static const Kernel kernels[2][2][2] = {{MV_ROW(false, false), MV_ROW(false, true)}, {MV_ROW(true, false), MV_ROW(true, true)}};
 #undef MV_ROW
-    const Kernel kernel = kernels[int4][sh][pairs >> 1];
+    const Kernel kernel = kernels[int4][paired][pairs - 1];
     if (smem > 32 * 1024) {  // with the fixed part more than a block has without asking
-        cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, MV_MAX_SMEM);
+        cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)(MV_SM_SMEM - 1024 - mv_static_bytes(pairs)));
         if (e != cudaSuccess)
             return launched("moe_b200_w4_matvec: shared memory", e);
     }
     const long long passes = ids ? n_rows : (n_rows + 2 * pairs - 1) / (2 * pairs);
-    const int fixed = 1024 + 2048 + 64 + 2 * pairs * 4 + pairs * 2048 + 1024;  // static shared memory and the system's
-    const long long fit = (228 * 1024) / ((long long)smem + fixed), occ = MV_BLOCKS;
-    const long long items = passes * a.n_tiles, most = (fit < 1 ? 1 : fit < occ ? fit : occ) * sms;
-    kernel<<<(unsigned)(items < most ? items : most), MV_THREADS, smem, st>>>(a);
+    const long long items = passes * a.n_tiles, most = (long long)blocks * sms;
+    kernel<<<(unsigned)(items < most ? items : most), MV_BLOCK, smem, st>>>(a);
     return launched("moe_b200_w4_matvec", cudaGetLastError());
 }
 

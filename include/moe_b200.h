@@ -478,7 +478,7 @@ typedef struct {
  *   out[m] = W[ids[m]] x[m / rows_per_x] + bias[ids[m]]     (ids NULL: the one matrix)
  * With the indices of a routing call and rows_per_x = K these are the experts'
  * products of n_rows / K tokens; a matrix that several rows ask for is read once
- * per 8 of them (4 or 2 for very long rows).  A row whose id is not in 0..n_mats-1
+ * per 2 or 4 of them.  A row whose id is not in 0..n_mats-1
  * (-1 of an empty slot) becomes zeros.
  *   x      [rows, cols] bf16 or f16, or e4m3 with x_scales of kind x_scale_kind (as
  *          moe_b200_add_rmsnorm writes them).  x_stride may be 0
@@ -486,8 +486,10 @@ typedef struct {
  *          SwiGLU of moe_b200_config (alpha, limit): g = min(gate, limit),
  *          u = clamp(up, +-limit), g sigmoid(alpha g) (u + 1)
  *   out    [n_rows, rows] (rows / 2 with swiglu) f32, bf16 or f16
- * Products are exact and summed in fp32; one rounding at the end.  Row addresses
- * of x must be 16-byte aligned (8 bytes for e4m3). */
+ * Products are exact and summed in fp32, a row's in an order that depends on cols
+ * alone; one rounding at the end.  Row addresses of x must be 16-byte aligned (8
+ * bytes for e4m3).  The kernel's waits for its own copies are bounded (2 s): rows
+ * behind one that ran out become NaN. */
 #define MOE_B200_W4_MATVEC_MAX_ROWS 256
 #define MOE_B200_W4_MATVEC_MAX_IN 16384
 #define MOE_B200_W4_MATVEC_MAX_OUT 4194304
