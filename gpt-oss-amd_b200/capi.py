@@ -52,11 +52,22 @@ class Config(ctypes.Structure):
     ]
 
 
-class W4Matrix(ctypes.Structure):
-    _fields_ = [
-        ("format", ctypes.c_int), ("group", ctypes.c_int), ("n_mats", ctypes.c_int), ("rows", ctypes.c_int),
-        ("cols", ctypes.c_int), ("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("bias", ctypes.c_void_p),
-    ]
+def _struct(name: str, **fields):
+    return type(name, (ctypes.Structure,), {"_fields_": list(fields.items())})
+
+
+_i, _f, _p, _ll = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_longlong
+AddRmsnormArgs = _struct(
+    "AddRmsnormArgs", n_rows=_i, hidden_dim=_i, x=_p, x_dtype=_i, x_stride=_ll, residual=_p, residual_dtype=_i,
+    residual_stride=_ll, residual_out=_p, residual_out_stride=_ll, weight=_p, weight_dtype=_i, eps=_f, y=_p, y_dtype=_i,
+    y_stride=_ll, q=_p, q_stride=_ll, q_scales=_p, q_kind=_i)
+RouteLogitsArgs = _struct(
+    "RouteLogitsArgs", n_tokens=_i, n_experts=_i, experts_per_token=_i, logits=_p, dtype=_i, stride=_ll, score=_i, bias=_p,
+    n_groups=_i, topk_groups=_i, group_top=_i, renormalize=_i, scale=_f, topk_i=_p, topk_w=_p, expert_counts=_p)
+W4Matrix = _struct("W4Matrix", format=_i, group=_i, n_mats=_i, rows=_i, cols=_i, codes=_p, scales=_p, bias=_p)
+W4MatvecArgs = _struct(
+    "W4MatvecArgs", w=W4Matrix, x=_p, x_dtype=_i, x_stride=_ll, x_scales=_p, x_scale_kind=_i, n_rows=_i, rows_per_x=_i,
+    ids=_p, swiglu=_i, swiglu_alpha=_f, swiglu_limit=_f, out=_p, out_dtype=_i, out_stride=_ll)
 
 
 class MoEError(RuntimeError):
@@ -100,10 +111,9 @@ def _bind(L: ctypes.CDLL) -> ctypes.CDLL:
     L.moe_b200_ep_peer_enable.argtypes = [vp, ctypes.c_char_p]
     L.moe_b200_ep_peer_sequence.argtypes = [vp]
     L.moe_b200_ep_peer_resync.argtypes = [vp, ci]
-    ll, cf = ctypes.c_longlong, ctypes.c_float
-    L.moe_b200_add_rmsnorm.argtypes = [vp, ci, ll, vp, ci, ll, vp, ll, vp, ci, cf, ci, ci, vp, ci, ll, vp, ll, vp, ci, vp]
-    L.moe_b200_route_logits.argtypes = [vp, ci, ll, ci, ci, ci, ci, vp, ci, ci, ci, ci, cf, vp, vp, vp, vp]
-    L.moe_b200_w4_matvec.argtypes = [ctypes.POINTER(W4Matrix), vp, ci, ll, vp, ci, ci, ci, vp, ci, cf, cf, vp, ci, ll, vp]
+    L.moe_b200_add_rmsnorm.argtypes = [ctypes.POINTER(AddRmsnormArgs), vp]
+    L.moe_b200_route_logits.argtypes = [ctypes.POINTER(RouteLogitsArgs), vp]
+    L.moe_b200_w4_matvec.argtypes = [ctypes.POINTER(W4MatvecArgs), vp]
     fp = ctypes.POINTER(ctypes.c_float)
     L.moe_b200_expert_file_info.argtypes = [ctypes.c_char_p, ip, ip, ip, ip, ip, fp,
                                             ctypes.POINTER(ctypes.c_ulonglong)]

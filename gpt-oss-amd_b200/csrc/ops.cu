@@ -66,11 +66,11 @@ bool rows_aligned(const void* p, long long stride, int size, size_t n) {
 
 extern "C" {
 
-moe_b200_status moe_b200_add_rmsnorm(const void* x, int x_dtype, long long x_stride, const void* residual,
-                                     int residual_dtype, long long residual_stride, void* residual_out,
-                                     long long residual_out_stride, const void* weight, int weight_dtype, float eps,
-                                     int n_rows, int hidden_dim, void* y, int y_dtype, long long y_stride, void* q,
-                                     long long q_stride, void* q_scales, int q_kind, moe_b200_stream stream) {
+moe_b200_status moe_b200_add_rmsnorm(const moe_b200_add_rmsnorm_args* args, moe_b200_stream stream) {
+    if (!args)
+        INVALID("moe_b200_add_rmsnorm: null pointer");
+    const auto [n_rows, hidden_dim, x, x_dtype, x_stride, residual, residual_dtype, residual_stride, residual_out,
+                residual_out_stride, weight, weight_dtype, eps, y, y_dtype, y_stride, q, q_stride, q_scales, q_kind] = *args;
     const int H = hidden_dim;
     if (n_rows < 0 || H <= 0 || H > MOE_B200_ADD_RMSNORM_MAX_HIDDEN)
         INVALID("moe_b200_add_rmsnorm: needs n_rows >= 0 and hidden_dim in 1..%d", MOE_B200_ADD_RMSNORM_MAX_HIDDEN);
@@ -128,10 +128,11 @@ moe_b200_status moe_b200_add_rmsnorm(const void* x, int x_dtype, long long x_str
     return launched("moe_b200_add_rmsnorm", cudaGetLastError());
 }
 
-moe_b200_status moe_b200_route_logits(const void* logits, int dtype, long long stride, int n_tokens, int n_experts,
-                                      int experts_per_token, int score, const float* bias, int n_groups,
-                                      int topk_groups, int group_top, int renormalize, float scale, int* topk_i,
-                                      float* topk_w, int* expert_counts, moe_b200_stream stream) {
+moe_b200_status moe_b200_route_logits(const moe_b200_route_logits_args* args, moe_b200_stream stream) {
+    if (!args)
+        INVALID("moe_b200_route_logits: null pointer");
+    const auto [n_tokens, n_experts, experts_per_token, logits, dtype, stride, score, bias, n_groups, topk_groups, group_top,
+                renormalize, scale, topk_i, topk_w, expert_counts] = *args;
     const int E = n_experts, K = experts_per_token;
     if (n_tokens < 0 || n_tokens > MOE_B200_ROUTE_LOGITS_MAX_TOKENS || E <= 0 || E > MOE_B200_ROUTE_LOGITS_MAX_EXPERTS)
         INVALID("moe_b200_route_logits: needs n_tokens in 0..%d and n_experts in 1..%d",
@@ -193,12 +194,12 @@ moe_b200_status moe_b200_route_logits(const void* logits, int dtype, long long s
     return launched("moe_b200_route_logits", cudaGetLastError());
 }
 
-moe_b200_status moe_b200_w4_matvec(const moe_b200_w4_matrix* w, const void* x, int x_dtype, long long x_stride,
-                                   const void* x_scales, int x_scale_kind, int n_rows, int rows_per_x, const int* ids,
-                                   int swiglu, float swiglu_alpha, float swiglu_limit, void* out, int out_dtype,
-                                   long long out_stride, moe_b200_stream stream) {
-    if (!w)
+moe_b200_status moe_b200_w4_matvec(const moe_b200_w4_matvec_args* args, moe_b200_stream stream) {
+    if (!args)
         INVALID("moe_b200_w4_matvec: null pointer");
+    const auto [matrix, x, x_dtype, x_stride, x_scales, x_scale_kind, n_rows, rows_per_x, ids, swiglu, swiglu_alpha,
+                swiglu_limit, out, out_dtype, out_stride] = *args;
+    const moe_b200_w4_matrix* w = &matrix;
     const bool int4 = w->format == MOE_B200_W4_INT4;
     if (!int4 && w->format != MOE_B200_W4_MXFP4)
         INVALID("moe_b200_w4_matvec: unknown weight format %d", w->format);

@@ -8,7 +8,6 @@ A wrong argument raises ``ValueError`` here or ``capi.MoEError`` with the librar
 """
 from __future__ import annotations
 
-import ctypes
 from typing import NamedTuple
 
 import torch
@@ -73,14 +72,14 @@ def _device(t):
     return dev
 
 
-def _call(name, dev, stream, *args):
+def _call(name, dev, stream, args):
     fn = getattr(capi.lib(), name)
     raw = torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
     if dev == torch._C._cuda_getDevice():
-        status = fn(*args, raw)
+        status = fn(args, raw)
     else:
         with torch.cuda.device(dev):
-            status = fn(*args, raw)
+            status = fn(args, raw)
     if status:
         capi.check(status)
 
@@ -126,8 +125,8 @@ def add_rmsnorm(x, weight, residual=None, *, eps=1e-5, dtype=torch.bfloat16, qua
         sp = _dense(q_scales, "q_scales", (T, n), _MX_TYPES if quant == "mx" else _F32, dev)
     elif q is not None or q_scales is not None:
         raise ValueError("q without quant")
-    _call("moe_b200_add_rmsnorm", dev, stream, xp, _FLOATS[x.dtype], xs, rp, rt, rs, rop, ros, wp, _FLOATS[weight.dtype], eps,
-          T, H, yp, yt, ys, qp, qs, sp, kind)
+    _call("moe_b200_add_rmsnorm", dev, stream, capi.AddRmsnormArgs(
+        T, H, xp, _FLOATS[x.dtype], xs, rp, rt, rs, rop, ros, wp, _FLOATS[weight.dtype], eps, yp, yt, ys, qp, qs, sp, kind))
     return NormResult(out, residual_out, q, q_scales)
 
 
@@ -164,8 +163,9 @@ def route_logits(logits, k, *, score="softmax", bias=None, n_groups=1, topk_grou
         counts = None
     if counts is not None:
         cp = _dense(counts, "counts", (E,), _I32, dev)
-    _call("moe_b200_route_logits", dev, stream, lp, _FLOATS[logits.dtype], ls, T, E, k, _SCORES[score], bp, n_groups,
-          topk_groups, group_top, bool(renormalize), scale, ip, wp, cp)
+    _call("moe_b200_route_logits", dev, stream, capi.RouteLogitsArgs(
+        T, E, k, lp, _FLOATS[logits.dtype], ls, _SCORES[score], bp, n_groups, topk_groups, group_top, bool(renormalize), scale,
+        ip, wp, cp))
     return Routing(topk_i, topk_w, counts)
 
 
@@ -223,6 +223,6 @@ def w4_matvec(x, codes, scales, bias=None, *, x_scales=None, ids=None, rows_per_
     op, os_ = _rows(out, "out", M, n_out, _FLOATS, dev)
     w = capi.W4Matrix(capi.W4_INT4 if scales.dtype == torch.bfloat16 else capi.W4_MXFP4, K // G, shape[0] if stack else 1, N, K,
                       cp, sp, bp)
-    _call("moe_b200_w4_matvec", dev, stream, ctypes.byref(w), xp, _X4[x.dtype], xs, xsp, kind, M, rows_per_x, ip,
-          swiglu is not None, alpha, limit, op, _FLOATS[out.dtype], os_)
+    _call("moe_b200_w4_matvec", dev, stream, capi.W4MatvecArgs(
+        w, xp, _X4[x.dtype], xs, xsp, kind, M, rows_per_x, ip, swiglu is not None, alpha, limit, op, _FLOATS[out.dtype], os_))
     return out

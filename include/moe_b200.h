@@ -411,49 +411,74 @@ moe_b200_status moe_b200_route_noalloc(const void* t, int t_dtype, int n_tokens,
  *   residual_out = r                                        optional
  *   y = r / sqrt(mean(r^2) + eps) * weight                  optional
  *   q = e4m3(y / scale), q_scales = scale                   optional
- * x [n_rows, H], residual, y f32, bf16 or f16; weight [H] of any of the three;
- * residual_out has residual's type.  All in fp32, each output rounded once; the
- * norm is of r before it is rounded to residual_out's type.  residual_out may be
- * residual itself; any output may be an input of the same type and stride; other
- * overlaps are the caller's error.
+ * All in fp32, each output rounded once; the norm is of r before it is rounded to
+ * residual_out's type.  residual_out may be residual itself; any output may be an
+ * input of the same type and stride; other overlaps are the caller's error.
  * A group's fp32 scale is its largest |y| / 448 (1 where that is 0, and not
  * below 2^-126); an MX scale is the least power of two s with largest |y| <= 448 s
  * (2^0 where that is 0, not below 2^-127).  Largest means of the numbers: NaN is
- * passed over there and becomes a NaN code.  Any H up to
- * MOE_B200_ADD_RMSNORM_MAX_HIDDEN, any stride; rows on 16-byte boundaries with H a
- * multiple of 8 take the fast path. */
+ * passed over there and becomes a NaN code.  Any hidden_dim up to
+ * MOE_B200_ADD_RMSNORM_MAX_HIDDEN, any stride; rows on 16-byte boundaries (8 for q)
+ * with hidden_dim a multiple of 8 take the fast path. */
 #define MOE_B200_ADD_RMSNORM_MAX_HIDDEN 32768
-moe_b200_status moe_b200_add_rmsnorm(const void* x, int x_dtype, long long x_stride, const void* residual,
-                                     int residual_dtype, long long residual_stride, void* residual_out,
-                                     long long residual_out_stride, const void* weight, int weight_dtype, float eps,
-                                     int n_rows, int hidden_dim, void* y, int y_dtype, long long y_stride, void* q,
-                                     long long q_stride, void* q_scales, int q_kind, moe_b200_stream stream);
+typedef struct {
+    int n_rows, hidden_dim;
+    const void* x;             /* [n_rows, hidden_dim] f32, bf16 or f16          */
+    int x_dtype;
+    long long x_stride;
+    const void* residual;      /* [n_rows, hidden_dim] or NULL                   */
+    int residual_dtype;        /* of residual and residual_out                   */
+    long long residual_stride;
+    void* residual_out;        /* or NULL                                        */
+    long long residual_out_stride;
+    const void* weight;        /* [hidden_dim] f32, bf16 or f16                  */
+    int weight_dtype;
+    float eps;
+    void* y;                   /* [n_rows, hidden_dim] f32, bf16 or f16, or NULL */
+    int y_dtype;
+    long long y_stride;
+    void* q;                   /* [n_rows, hidden_dim] e4m3, or NULL             */
+    long long q_stride;
+    void* q_scales;
+    int q_kind;                /* MOE_B200_SCALE_ROW .. MOE_B200_SCALE_MX        */
+} moe_b200_add_rmsnorm_args;
+moe_b200_status moe_b200_add_rmsnorm(const moe_b200_add_rmsnorm_args* args, moe_b200_stream stream);
 
-/* Experts and weights from router logits [n_tokens, n_experts] (f32, bf16, f16):
+/* Experts and weights from router logits:
  *   p_e   = softmax over the experts, or the sigmoid, of the logits
- *   key_e = p_e + bias_e with a bias (f32 [n_experts], for balance: it moves the
- *           choice, not the weights); without one the order of the logits
+ *   key_e = p_e + bias_e with a bias (for balance: it moves the choice, not the
+ *           weights); without one the order of the logits
  *   groups: with n_groups > 1 the experts form n_groups equal neighbouring groups,
  *           scored by the sum of their group_top (1 or 2) largest keys (of p_e
  *           where there is no bias); experts of the topk_groups best take part
- *   topk_i = the K experts of the largest keys in falling order, ties (of experts
- *           and of groups) to the lower index
+ *   topk_i = the experts_per_token experts of the largest keys in falling order,
+ *           ties (of experts and of groups) to the lower index
  *   topk_w = p of the selected, divided by their sum when renormalize != 0, times
  *           scale.  softmax with renormalize is the softmax over the selected.
  * The order is that of keys computed in 64 bits.  An expert whose logit (or bias)
- * is -inf or NaN takes no part: softmax and groups do not count it, and a slot for
- * which no expert is left gets index -1 and weight 0.  +inf counts as the largest
- * finite value.  expert_counts (optional, [n_experts]): slots that went to each
- * expert, overwritten. */
+ * is -inf or NaN takes no part: softmax and groups do not count it (a bias of -inf:
+ * groups do not), and a slot for which no expert is left gets index -1 and weight
+ * 0.  +inf counts as the largest finite value. */
 #define MOE_B200_SCORE_SOFTMAX 0
 #define MOE_B200_SCORE_SIGMOID 1
 #define MOE_B200_ROUTE_LOGITS_MAX_TOKENS 16777216
 #define MOE_B200_ROUTE_LOGITS_MAX_EXPERTS 512
 #define MOE_B200_ROUTE_LOGITS_MAX_K 16
-moe_b200_status moe_b200_route_logits(const void* logits, int dtype, long long stride, int n_tokens, int n_experts,
-                                      int experts_per_token, int score, const float* bias, int n_groups,
-                                      int topk_groups, int group_top, int renormalize, float scale, int* topk_i,
-                                      float* topk_w, int* expert_counts, moe_b200_stream stream);
+typedef struct {
+    int n_tokens, n_experts, experts_per_token;
+    const void* logits;   /* [n_tokens, n_experts] f32, bf16 or f16              */
+    int dtype;
+    long long stride;
+    int score;            /* MOE_B200_SCORE_SOFTMAX or MOE_B200_SCORE_SIGMOID    */
+    const float* bias;    /* [n_experts] or NULL                                 */
+    int n_groups, topk_groups, group_top; /* 1, 1, any: no groups                */
+    int renormalize;
+    float scale;
+    int* topk_i;          /* [n_tokens, experts_per_token]                       */
+    float* topk_w;        /* [n_tokens, experts_per_token]                       */
+    int* expert_counts;   /* [n_experts] slots that went to each expert, or NULL */
+} moe_b200_route_logits_args;
+moe_b200_status moe_b200_route_logits(const moe_b200_route_logits_args* args, moe_b200_stream stream);
 
 /* A stack of matrices in 4 bits.  Two codes per byte, the even column in the low
  * half; codes 16-byte aligned.
@@ -493,10 +518,22 @@ typedef struct {
 #define MOE_B200_W4_MATVEC_MAX_ROWS 256
 #define MOE_B200_W4_MATVEC_MAX_IN 16384
 #define MOE_B200_W4_MATVEC_MAX_OUT 4194304
-moe_b200_status moe_b200_w4_matvec(const moe_b200_w4_matrix* w, const void* x, int x_dtype, long long x_stride,
-                                   const void* x_scales, int x_scale_kind, int n_rows, int rows_per_x, const int* ids,
-                                   int swiglu, float swiglu_alpha, float swiglu_limit, void* out, int out_dtype,
-                                   long long out_stride, moe_b200_stream stream);
+typedef struct {
+    moe_b200_w4_matrix w;
+    const void* x;         /* [ceil(n_rows / rows_per_x), cols]                  */
+    int x_dtype;
+    long long x_stride;
+    const void* x_scales;
+    int x_scale_kind;
+    int n_rows, rows_per_x;
+    const int* ids;        /* [n_rows] or NULL                                   */
+    int swiglu;
+    float swiglu_alpha, swiglu_limit;
+    void* out;             /* [n_rows, rows] or [n_rows, rows / 2]               */
+    int out_dtype;
+    long long out_stride;
+} moe_b200_w4_matvec_args;
+moe_b200_status moe_b200_w4_matvec(const moe_b200_w4_matvec_args* args, moe_b200_stream stream);
 
 /* Library build info, e.g. "moe_b200 0.1 sm_100a". */
 const char* moe_b200_version(void);

@@ -1,7 +1,5 @@
 """The stand-alone operators refuse wrong arguments with a status and a text, before anything is launched:
 no GPU is needed (the pointers below are never followed)."""
-import ctypes
-
 import pytest
 import torch
 
@@ -12,17 +10,17 @@ A = 4096  # an aligned address
 
 
 def _norm(**kw):
-    a = dict(x=A, xt=capi.DTYPE_BF16, xs=64, r=A, rt=capi.DTYPE_F32, rs=64, ro=A, ros=64, w=A, wt=capi.DTYPE_F32, eps=1e-5,
-             T=4, H=64, y=A, yt=capi.DTYPE_BF16, ys=64, q=A, qs=64, sc=A, kind=capi.SCALE_ROW)
+    a = dict(T=4, H=64, x=A, xt=capi.DTYPE_BF16, xs=64, r=A, rt=capi.DTYPE_F32, rs=64, ro=A, ros=64, w=A, wt=capi.DTYPE_F32,
+             eps=1e-5, y=A, yt=capi.DTYPE_BF16, ys=64, q=A, qs=64, sc=A, kind=capi.SCALE_ROW)
     a.update(kw)
-    return capi.lib().moe_b200_add_rmsnorm(*a.values(), None)
+    return capi.lib().moe_b200_add_rmsnorm(capi.AddRmsnormArgs(*a.values()), None)
 
 
 def _route(**kw):
-    a = dict(l=A, dt=capi.DTYPE_F32, s=64, T=4, E=64, K=4, score=capi.SCORE_SOFTMAX, bias=None, ng=1, kg=1, gt=1, rn=1, scale=1.0,
+    a = dict(T=4, E=64, K=4, l=A, dt=capi.DTYPE_F32, s=64, score=capi.SCORE_SOFTMAX, bias=None, ng=1, kg=1, gt=1, rn=1, scale=1.0,
              i=A, w=A, c=None)
     a.update(kw)
-    return capi.lib().moe_b200_route_logits(*a.values(), None)
+    return capi.lib().moe_b200_route_logits(capi.RouteLogitsArgs(*a.values()), None)
 
 
 def _matvec(mat=None, **kw):
@@ -31,8 +29,13 @@ def _matvec(mat=None, **kw):
     a = dict(x=A, xt=capi.DTYPE_BF16, xs=64, sc=None, kind=capi.SCALE_NONE, M=4, rpx=1, ids=None, sw=0, al=1.702, li=7.0, out=A,
              ot=capi.DTYPE_BF16, os=64)
     a.update(kw)
-    w = capi.W4Matrix(**m)
-    return capi.lib().moe_b200_w4_matvec(ctypes.byref(w), *a.values(), None)
+    return capi.lib().moe_b200_w4_matvec(capi.W4MatvecArgs(capi.W4Matrix(**m), *a.values()), None)
+
+
+def test_null_arguments_are_refused():
+    L = capi.lib()
+    for fn in (L.moe_b200_add_rmsnorm, L.moe_b200_route_logits, L.moe_b200_w4_matvec):
+        assert fn(None, None) == capi.ERR_INVALID
 
 
 @pytest.mark.parametrize("kw", [
