@@ -382,8 +382,11 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) route_logits_kernel(const __
             if (!(by_logit && a.group_top == 1) && a.topk_groups < a.n_groups) {
                 const float low = -warp_best(in && g < a.n_groups ? -score : -INFINITY);
                 const float high = warp_best(!in && g < a.n_groups ? score : -INFINITY);
+                // a score is off by its two keys' errors and a rounding; the keys may be far larger than their sum
+                const float big = warp_best(fmaxf(group_best > -INFINITY ? fabsf(group_best) : 0.f,
+                                                  group_next > -INFINITY ? fabsf(group_next) : 0.f));
                 if (high > -INFINITY)
-                    sure = low - high > 2.f * tol_p + 2.f * HALF_STEP2 * fmaxf(fabsf(low), fabsf(high));
+                    sure = low - high > 2.f * tol_p + 4.f * HALF_STEP2 * big;
             }
             if (lanes_of_group) {
                 if (!in) {

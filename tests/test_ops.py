@@ -250,6 +250,18 @@ def test_route_logits_keys_closer_than_fp32():
     _check_route(logits, k, pkg.route_logits(logits, k, **kw), **kw)
 
 
+def test_route_logits_groups_of_keys_that_cancel():
+    """Group scores that are small sums of large keys: fp32 loses them, the choice is that of 64 bits."""
+    g = _gen(12)
+    T, E, k = 64, 64, 8
+    logits = 2.0**-12 * _randn(g, T, E)
+    bias = torch.full((E,), -5000.0, device="cuda")
+    bias[::8] = 5000.0  # the best of each group; its second best is -5000 + p
+    for G in (8, 4):
+        kw = dict(score="sigmoid", bias=bias, n_groups=G, topk_groups=G // 2, group_top=2)
+        _check_route(logits, k, pkg.route_logits(logits, k, **kw), **kw)
+
+
 def test_route_logits_large_batch_strides_and_rows_behind():
     """Many tokens per warp; every expert id of a large batch against the small-batch call, nothing written behind."""
     g = _gen(8)
