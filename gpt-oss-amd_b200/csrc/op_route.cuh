@@ -21,7 +21,6 @@
 #include <float.h>
 
 #include <type_traits>
-#include <utility>
 
 #include "op_types.cuh"
 
@@ -73,7 +72,7 @@ __device__ __forceinline__ float warp_best(float v) {
 }
 
 // The logit that takes part: NaN and -inf do not (-inf), +inf is the largest finite value.
-__device__ __forceinline__ float route_logit(float v) { return v > -INFINITY ? fminf(v, FLT_MAX) : -INFINITY; }
+__device__ __forceinline__ float route_logit(float v) { return fminf(fmaxf(v, -INFINITY), FLT_MAX); }
 
 // One token with 64-bit keys, from the definition and without hurry: `keys` holds E values of shared memory of
 // this warp.  Returns the expert of slot `lane`, -1 where there is none.
@@ -148,64 +147,49 @@ __device__ __noinline__ int route_exact(const LogitsArgs& a, long long t, float 
     return mine;
 }
 
-constexpr int ROUTE_WARPS = 16;
-
-// The exchanges of Batcher's odd-even merge sort of NT places, in order.
-template <int NT>
-struct SortNetwork {
-    int x[NT * NT], y[NT * NT], n;
-    constexpr SortNetwork() : x{}, y{}, n(0) {
-        for (int p = 1; p < NT; p *= 2)
-            for (int k = p; k >= 1; k /= 2)
-                for (int j = k % p; j + k < NT; j += 2 * k)
-                    for (int i = 0; i < k && i + j + k < NT; i++)
-                        if ((i + j) / (2 * p) == (i + j + k) / (2 * p)) {
-                            x[n] = i + j;
-                            y[n] = i + j + k;
-                            n++;
-                        }
-    }
-};
-
-template <int NT, int... I>
-__device__ __forceinline__ void sort_exchanges(float (&key)[NT], int (&idx)[NT], std::integer_sequence<int, I...>) {
-    constexpr SortNetwork<NT> net;
-    auto exchange = [&](int x, int y) {
-        const bool swap = key[y] > key[x] || (key[y] == key[x] && idx[y] < idx[x]);
-        const float kx = swap ? key[y] : key[x], ky = swap ? key[x] : key[y];
-        const int ix = swap ? idx[y] : idx[x], iy = swap ? idx[x] : idx[y];
-        key[x] = kx;
-        key[y] = ky;
-        idx[x] = ix;
-        idx[y] = iy;
-    };
-    (exchange(std::integral_constant<int, net.x[I]>::value, std::integral_constant<int, net.y[I]>::value), ...);
+// In fp32, 0 for -inf: relative error 2^-21 + |x| 2^-23 at most.
+__device__ __forceinline__ float route_sigmoid(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-x)));
+    return r;
 }
 
-// Sorts the keys of a lane in falling order, ties by index; perm: four bits per place, the index within the lane.
-template <int NT, typename Perm>
-__device__ __forceinline__ void sort_lane(float (&key)[NT], Perm& perm) {
-    int idx[NT];
+constexpr int ROUTE_WARPS = 16;
+
+// Places of a lane's keys in falling order, ties by index, four bits each: a key's place is the number of keys
+// in front of it, and a comparison of two moves one of them a place back.
+template <int NT>
+__device__ __forceinline__ void places_of(const float (&key)[NT], int (&place)[NT]) {
+    typedef typename std::conditional<NT == 16, unsigned long long, unsigned>::type Packed;
+    Packed packed = 0;
 #pragma unroll
-    for (int j = 0; j < NT; j++)
-        idx[j] = j;
-    constexpr SortNetwork<NT> net;
-    sort_exchanges<NT>(key, idx, std::make_integer_sequence<int, net.n>{});
-    perm = 0;
+    for (int i = 0; i < NT; i++)
+        packed |= (Packed)(NT - 1 - i) << (4 * i);
 #pragma unroll
-    for (int j = 0; j < NT; j++)
-        perm |= (Perm)idx[j] << (4 * j);
+    for (int j = 1; j < NT; j++)
+#pragma unroll
+        for (int i = 0; i < j; i++)
+            if (key[i] >= key[j])
+                packed += ((Packed)1 << (4 * j)) - ((Packed)1 << (4 * i));
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+        place[i] = (int)(packed >> (4 * i)) & 15;
+}
+
+// Dynamic shared memory of a warp: its keys in order, and route_exact's.
+template <int NT>
+__host__ __device__ constexpr size_t route_smem_bytes() {
+    return (NT + 1) * 32 * sizeof(float2) + NT * 32 * sizeof(double);
 }
 
 // VEC: a lane's logits are one aligned piece of memory.
 template <int NT, bool VEC>
 __global__ void __launch_bounds__(32 * ROUTE_WARPS) route_logits_kernel(const __grid_constant__ LogitsArgs a) {
-    typedef typename std::conditional<NT == 16, unsigned long long, unsigned>::type Perm;
-    __shared__ float s_sorted[ROUTE_WARPS][NT + 1][32];  // place, lane
     __shared__ int s_sel[ROUTE_WARPS][32];
-    extern __shared__ double s_keys_all[];  // [warps][32 * NT]
+    extern __shared__ double s_dyn[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    double* s_keys = s_keys_all + warp * 32 * NT;
+    float2(*sorted)[32] = reinterpret_cast<float2(*)[32]>(s_dyn + warp * (route_smem_bytes<NT>() / 8));  // place, lane
+    double* s_keys = reinterpret_cast<double*>(sorted + NT + 1);
     if (a.counts && blockIdx.x == 0)
         for (int i = threadIdx.x; i < a.E; i += blockDim.x)
             a.counts[i] = 0;  // route_counts_kernel adds to them
@@ -221,8 +205,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) route_logits_kernel(const __
         const float b = a.bias && e < a.E ? a.bias[e] : 0.f;
         bias[j] = b > -INFINITY ? fminf(b, FLT_MAX) : -INFINITY;
     }
-    float(*sorted)[32] = s_sorted[warp];
-    sorted[NT][lane] = -INFINITY;
+    sorted[NT][lane] = make_float2(-INFINITY, 0.f);
     int* sel = s_sel[warp];
     for (int t = blockIdx.x * (blockDim.x >> 5) + warp; t < a.T; t += gridDim.x * (blockDim.x >> 5)) {
         float l[NT];
@@ -282,7 +265,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) route_logits_kernel(const __
             if (a.sigmoid) {
 #pragma unroll
                 for (int j = 0; j < NT; j++)  // 0 for -inf
-                    key[j] = __fdividef(1.f, 1.f + __expf(-l[j]));
+                    key[j] = route_sigmoid(l[j]);
             } else {
 #pragma unroll
                 for (int j = 0; j < NT; j++) {
@@ -291,6 +274,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) route_logits_kernel(const __
                 }
                 sum = warp_sum(sum);
                 const float inv = 1.f / sum;
+                pmax = inv;
 #pragma unroll
                 for (int j = 0; j < NT; j++)
                     key[j] *= inv;
@@ -301,15 +285,11 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) route_logits_kernel(const __
         // reciprocal and product, 20 for a softmax's sum of up to 512 terms in a tree; p + bias by one of the sum's.
         float tol_p = 0.f;
         if (need_p) {
-#pragma unroll
-            for (int j = 0; j < NT; j++)
-                pmax = fmaxf(pmax, key[j]);
-            pmax = warp_best(pmax);
+            pmax = a.sigmoid ? route_sigmoid(lmax) : pmax;
             tol_p = 2.f * 5.97e-8f * ((a.sigmoid ? 12.f : 32.f) + 2.f * fmaxf(1.f, a.sigmoid ? -lmax : 1.f)) * pmax;
         }
         constexpr float HALF_STEP2 = 2.f * 5.97e-8f;
         bool sure = true;
-        Perm perm;
         float group_best = 0.f, group_next = 0.f;  // of this lane's experts, by what scores groups
         if (by_logit) {
             if (need_p) {  // the two best p of the lane are those of its two best logits
@@ -341,16 +321,19 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) route_logits_kernel(const __
             for (int j = 0; j < NT; j++)
                 s_keys[lane * NT + j] = key[j];
         }
-        sort_lane<NT, Perm>(key, perm);
+        {
+            int place[NT];
+            places_of<NT>(key, place);
 #pragma unroll
-        for (int j = 0; j < NT; j++)
-            sorted[j][lane] = key[j];
+            for (int j = 0; j < NT; j++)
+                sorted[place[j]][lane] = make_float2(key[j], __int_as_float(lane * NT + j));
+        }
         __syncwarp();
 
         if (a.n_groups > 1) {
             if (!by_logit || !need_p) {
-                group_best = key[0];
-                group_next = NT > 1 ? key[NT > 1 ? 1 : 0] : -INFINITY;
+                group_best = sorted[0][lane].x;
+                group_next = sorted[1][lane].x;  // NT = 1: -inf
             }
             int g = lane;  // the group whose score this lane has
             if (lanes_of_group) {
@@ -389,50 +372,38 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) route_logits_kernel(const __
                     sure = low - high > 2.f * tol_p + 4.f * HALF_STEP2 * big;
             }
             if (lanes_of_group) {
-                if (!in) {
-                    key[0] = -INFINITY;
-#pragma unroll
-                    for (int j = 0; j < NT; j++)
-                        sorted[j][lane] = -INFINITY;
-                }
+                if (!in)
+                    sorted[0][lane].x = -INFINITY;
             } else {
                 const unsigned kept = __ballot_sync(0xffffffffu, in);
-#pragma unroll
-                for (int j = 0; j < NT; j++) {  // in falling order again
-                    const int e = lane * NT + (int)((perm >> (4 * j)) & 15u);
-                    key[j] = e < a.E && ((kept >> (e / gs)) & 1u) ? sorted[j][lane] : -INFINITY;
-                }
-                Perm order = 0;
                 int n = 0;
-#pragma unroll
-                for (int j = 0; j < NT; j++)
-                    if (key[j] > -INFINITY) {
-                        sorted[n][lane] = key[j];
-                        order |= ((perm >> (4 * j)) & 15u) << (4 * n);
-                        n++;
-                    }
+#pragma unroll 1
+                for (int j = 0; j < NT; j++) {  // those that stay move up
+                    const float2 v = sorted[j][lane];
+                    const int e = __float_as_int(v.y);
+                    if (v.x > -INFINITY && e < a.E && ((kept >> (e / gs)) & 1u))
+                        sorted[n++][lane] = v;
+                }
                 for (int j = n; j < NT; j++)
-                    sorted[j][lane] = -INFINITY;
-                perm = order;
-                key[0] = sorted[0][lane];
+                    sorted[j][lane].x = -INFINITY;
             }
         }
 
         // Rounds: the largest head, of the lowest lane that has it; that lane leaves the expert in `sel` and
         // moves on.  Lane k keeps the key of round k.
-        float head = key[0], mine_key = -INFINITY;
-        const float* next = &sorted[1][lane];
+        float2 head = sorted[0][lane];
+        float mine_key = -INFINITY;
+        const float2* next = &sorted[1][lane];
         const unsigned lower = (1u << lane) - 1u;
         auto round = [&](int k) {
-            const float top = warp_best(head);
-            const unsigned has = __ballot_sync(0xffffffffu, head == top);
+            const float top = warp_best(head.x);
+            const unsigned has = __ballot_sync(0xffffffffu, head.x == top);
             if (lane == k)
                 mine_key = top;
-            if (head == top && top > -INFINITY && !(has & lower)) {  // at most NT times: place NT holds -inf
-                sel[k] = lane * NT + (int)(perm & 15u);
+            if (head.x == top && top > -INFINITY && !(has & lower)) {  // at most NT times: place NT holds -inf
+                sel[k] = __float_as_int(head.y);
                 head = *next;
                 next += 32;
-                perm >>= 4;
             }
             return top;
         };

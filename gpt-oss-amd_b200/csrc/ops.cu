@@ -180,9 +180,12 @@ moe_b200_status moe_b200_route_logits(const moe_b200_route_logits_args* args, mo
                   : nt == 4 ? (vec ? route_logits_kernel<4, true> : route_logits_kernel<4, false>)
                   : nt == 8 ? (vec ? route_logits_kernel<8, true> : route_logits_kernel<8, false>)
                             : (vec ? route_logits_kernel<16, true> : route_logits_kernel<16, false>);
-    const size_t smem = sizeof(double) * 32 * nt * warps;
-    if (nt >= 8 && smem > 16 * 1024) {  // with the fixed part more than a block has without asking
-        cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024);
+    const size_t per_warp = nt == 1 ? route_smem_bytes<1>() : nt == 2 ? route_smem_bytes<2>() : nt == 4 ? route_smem_bytes<4>()
+                            : nt == 8 ? route_smem_bytes<8>() : route_smem_bytes<16>();
+    const size_t smem = per_warp * warps;
+    if (smem > 44 * 1024) {  // with the fixed part more than a block has without asking
+        cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)(per_warp * ROUTE_WARPS));
         if (e != cudaSuccess)
             return launched("moe_b200_route_logits: shared memory", e);
     }
