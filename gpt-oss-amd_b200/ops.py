@@ -72,9 +72,15 @@ def _device(t):
     return dev
 
 
-def _call(name, dev, stream, args):
+def _on(stream, fn, *args, **kw):
+    """The call with `stream` as the current one: new results come from that stream's memory."""
+    with torch.cuda.stream(stream):
+        return fn(*args, **kw)
+
+
+def _call(name, dev, args):
     fn = getattr(capi.lib(), name)
-    raw = torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
+    raw = torch._C._cuda_getCurrentRawStream(dev)
     if dev == torch._C._cuda_getDevice():
         status = fn(args, raw)
     else:
@@ -93,6 +99,9 @@ def add_rmsnorm(x, weight, residual=None, *, eps=1e-5, dtype=torch.bfloat16, qua
     be ``residual`` itself), in residual's type.  ``quant``: "row", 32, 64 or 128 (fp32 scales per row or
     group of columns) or "mx" (e8m0 per 32): q is float8_e4m3fn [T, H], q_scales [T, scales per row]
     float32, with "mx" float8_e8m0fnu (uint8 is taken too)."""
+    if stream is not None:
+        return _on(stream, add_rmsnorm, x, weight, residual, eps=eps, dtype=dtype, quant=quant, residual_out=residual_out,
+                   out=out, q=q, q_scales=q_scales)
     dev = _device(x)
     _need(x.dim() == 2, "x: needs two dimensions")
     T, H = x.shape
@@ -125,7 +134,7 @@ def add_rmsnorm(x, weight, residual=None, *, eps=1e-5, dtype=torch.bfloat16, qua
         sp = _dense(q_scales, "q_scales", (T, n), _MX_TYPES if quant == "mx" else _F32, dev)
     elif q is not None or q_scales is not None:
         raise ValueError("q without quant")
-    _call("moe_b200_add_rmsnorm", dev, stream, capi.AddRmsnormArgs(
+    _call("moe_b200_add_rmsnorm", dev, capi.AddRmsnormArgs(
         T, H, xp, _FLOATS[x.dtype], xs, rp, rt, rs, rop, ros, wp, _FLOATS[weight.dtype], eps, yp, yt, ys, qp, qs, sp, kind))
     return NormResult(out, residual_out, q, q_scales)
 
@@ -144,6 +153,9 @@ def route_logits(logits, k, *, score="softmax", bias=None, n_groups=1, topk_grou
     ``scale`` multiplies them.  Ties go to the lower index.  Experts with a logit of -inf or NaN take no
     part; empty slots have index -1 and weight 0.  ``counts``: True or an int32 [E] tensor for the number
     of slots per expert.  ``topk_i``, ``topk_w``: where the results go."""
+    if stream is not None:
+        return _on(stream, route_logits, logits, k, score=score, bias=bias, n_groups=n_groups, topk_groups=topk_groups,
+                   group_top=group_top, renormalize=renormalize, scale=scale, counts=counts, topk_i=topk_i, topk_w=topk_w)
     dev = _device(logits)
     _need(logits.dim() == 2, "logits: needs two dimensions")
     T, E = logits.shape
@@ -163,7 +175,7 @@ def route_logits(logits, k, *, score="softmax", bias=None, n_groups=1, topk_grou
         counts = None
     if counts is not None:
         cp = _dense(counts, "counts", (E,), _I32, dev)
-    _call("moe_b200_route_logits", dev, stream, capi.RouteLogitsArgs(
+    _call("moe_b200_route_logits", dev, capi.RouteLogitsArgs(
         T, E, k, lp, _FLOATS[logits.dtype], ls, _SCORES[score], bp, n_groups, topk_groups, group_top, bool(renormalize), scale,
         ip, wp, cp))
     return Routing(topk_i, topk_w, counts)
@@ -180,6 +192,9 @@ def w4_matvec(x, codes, scales, bias=None, *, x_scales=None, ids=None, rows_per_
     int32 [M], one matrix per row of the result, an index outside the stack gives zeros; without
     it M = x rows * rows_per_x.  ``swiglu``: (alpha, limit) for the framework's clamped SwiGLU over
     interleaved gate and up rows.  At most 256 rows."""
+    if stream is not None:
+        return _on(stream, w4_matvec, x, codes, scales, bias, x_scales=x_scales, ids=ids, rows_per_x=rows_per_x, swiglu=swiglu,
+                   out=out, dtype=dtype)
     dev = _device(x)
     _need(x.dim() == 2, "x: needs two dimensions")
     rows, K = x.shape
@@ -223,6 +238,6 @@ def w4_matvec(x, codes, scales, bias=None, *, x_scales=None, ids=None, rows_per_
     op, os_ = _rows(out, "out", M, n_out, _FLOATS, dev)
     w = capi.W4Matrix(capi.W4_INT4 if scales.dtype == torch.bfloat16 else capi.W4_MXFP4, K // G, shape[0] if stack else 1, N, K,
                       cp, sp, bp)
-    _call("moe_b200_w4_matvec", dev, stream, capi.W4MatvecArgs(
+    _call("moe_b200_w4_matvec", dev, capi.W4MatvecArgs(
         w, xp, _X4[x.dtype], xs, xsp, kind, M, rows_per_x, ip, swiglu is not None, alpha, limit, op, _FLOATS[out.dtype], os_))
     return out

@@ -566,6 +566,56 @@ def test_other_streams_and_overlapping_calls():
     assert torch.equal(r.y, pkg.add_rmsnorm(x, p["w"]).y)
 
 
+def test_stream_argument_of_every_operator():
+    """Results on a stream of the caller's, freshly allocated while the current stream still works on freed memory."""
+    shape = pkg.MoEShape(hidden=576, intermediate=320, n_experts=32, top_k=4)
+    _, p = _layer(shape, 4)
+    g = _gen(5)
+    x, res = _randn(g, 8, 576), _randn(g, 8, 576)
+    n0 = pkg.add_rmsnorm(x, p["w"], res, quant="mx")
+    r0 = pkg.route_logits(x[:, :32].contiguous(), 4, counts=True)
+    h0 = pkg.w4_matvec(n0.y, p["c1"], p["s1"], p["b1"], ids=r0.topk_i.view(-1), rows_per_x=4)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    n = pkg.add_rmsnorm(x, p["w"], res, quant="mx", stream=s)
+    s.synchronize()
+    r = pkg.route_logits(x[:, :32].contiguous(), 4, counts=True, stream=s)
+    s.synchronize()
+    h = pkg.w4_matvec(n.y, p["c1"], p["s1"], p["b1"], ids=r.topk_i.view(-1), rows_per_x=4, stream=s)
+    s.synchronize()
+    for a, b in zip((*n0, *r0, h0), (*n, *r, h)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_offsets_beyond_32_bits():
+    """The last rows of tensors of more than 2^31 elements or bytes."""
+    g = _gen(14)
+    T, H = 66000, 32768  # 2.16e9 elements
+    x = torch.zeros(T, H, dtype=BF16, device="cuda")
+    x[-3:] = _randn(g, 3, H).to(BF16)
+    w = torch.ones(H, dtype=BF16, device="cuda")
+    r = pkg.add_rmsnorm(x, w, quant="row")
+    _check_norm(x[-3:], w, None, type(r)(r.y[-3:], None, r.q[-3:], r.q_scales[-3:]), "row")
+    assert (r.y[:2] == 0).all()
+    del x, r
+    T, E = 4200000, 512  # 2.15e9 logits
+    logits = torch.zeros(T, E, dtype=F16, device="cuda")
+    logits[-5:] = _randn(g, 5, E).to(F16)
+    r = pkg.route_logits(logits, 6, counts=True)
+    _check_route(logits[-5:], 6, type(r)(r.topk_i[-5:], r.topk_w[-5:], None))
+    assert torch.equal(r.topk_i[:3].cpu(), torch.arange(6, dtype=torch.int32).repeat(3, 1)) and int(r.counts.sum()) == T * 6
+    del logits, r
+    n, N, K = 300, 5760, 2880  # 2.5e9 bytes of codes
+    codes = torch.zeros(n, N, K // 2, dtype=torch.uint8, device="cuda")
+    scales = torch.full((n, N, K // 32), 127, dtype=torch.uint8, device="cuda")
+    codes[-1], scales[-1] = _weights(g, (), N, K, "mxfp4", 32)
+    x, _, x64 = _x(g, 1, K, BF16)
+    ids = torch.tensor([n - 1, 0], dtype=torch.int32, device="cuda")
+    y = pkg.w4_matvec(x, codes, scales, ids=ids, rows_per_x=2, dtype=F32)
+    _check_matvec(y[:1], x64, codes[-1], scales[-1], None, 32, None, 1)
+    assert (y[1] == 0).all()
+
+
 def test_captured_and_replayed():
     """The whole step in a CUDA graph, two graphs of it replayed in turn on new inputs."""
     shape = pkg.MoEShape(hidden=576, intermediate=320, n_experts=32, top_k=4)
