@@ -16,9 +16,13 @@ from . import capi
 
 _FLOATS = {torch.float32: capi.DTYPE_F32, torch.bfloat16: capi.DTYPE_BF16, torch.float16: capi.DTYPE_F16}
 _X4 = {torch.bfloat16: capi.DTYPE_BF16, torch.float16: capi.DTYPE_F16, torch.float8_e4m3fn: capi.DTYPE_E4M3}
+_PACK_NORM = capi.packer(capi.AddRmsnormArgs)
+_PACK_ROUTE = capi.packer(capi.RouteLogitsArgs)
+_PACK_MATVEC = capi.packer(capi.W4MatvecArgs)
 _QUANT = {"row": capi.SCALE_ROW, 32: capi.SCALE_G32, 64: capi.SCALE_G64, 128: capi.SCALE_G128, "mx": capi.SCALE_MX}
 _MX_TYPES = (torch.float8_e8m0fnu, torch.uint8)
-_F32, _I32, _U8, _E4M3 = (torch.float32,), (torch.int32,), (torch.uint8,), (torch.float8_e4m3fn,)
+_F32, _I32, _U8 = (torch.float32,), (torch.int32,), (torch.uint8,)
+_E4M3 = {torch.float8_e4m3fn: capi.DTYPE_E4M3}
 _W4_SCALES, _X_SCALES = (torch.bfloat16, *_MX_TYPES), (torch.float32, *_MX_TYPES)
 
 
@@ -48,17 +52,19 @@ def _wrong(t, name, shape, types, dev, what):
                      f"got {tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
 
 
-def _rows(t, name, rows, cols, types, dev):
-    """Checks a 2-d tensor with neighbouring columns; returns its address and row stride."""
-    if t.dtype not in types or t.get_device() != dev or t.shape != (rows, cols):
-        _wrong(t, name, (rows, cols), types, dev, "contiguous rows of")
+def _rows(t, name, shape, types, dev):
+    """Checks a 2-d tensor with neighbouring columns; returns its address, its type's code and its row stride."""
+    code = types.get(t.dtype)
+    if code is None or t.get_device() != dev or t.shape != shape:
+        _wrong(t, name, shape, types, dev, "contiguous rows of")
     stride, one = t.stride()
-    if one != 1 and cols > 1:
-        _wrong(t, name, (rows, cols), types, dev, "contiguous rows of")
-    return t.data_ptr(), stride
+    if one != 1 and shape[1] > 1:
+        _wrong(t, name, shape, types, dev, "contiguous rows of")
+    return t.data_ptr(), code, stride
 
 
 def _dense(t, name, shape, types, dev):
+    """Checks a contiguous tensor; returns its address."""
     if t.dtype not in types or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
         _wrong(t, name, shape, types, dev, "contiguous")
     return t.data_ptr()
@@ -104,38 +110,39 @@ def add_rmsnorm(x, weight, residual=None, *, eps=1e-5, dtype=torch.bfloat16, qua
                    out=out, q=q, q_scales=q_scales)
     dev = _device(x)
     _need(x.dim() == 2, "x: needs two dimensions")
-    T, H = x.shape
-    xp, xs = _rows(x, "x", T, H, _FLOATS, dev)
+    shape = x.shape
+    T, H = shape
+    xp, xt, xs = _rows(x, "x", shape, _FLOATS, dev)
     wp = _dense(weight, "weight", (H,), _FLOATS, dev)
-    rp = rop = yp = qp = sp = None
-    rt = rs = ros = yt = ys = qs = kind = 0
+    rp = rop = yp = qp = sp = rt = rs = ros = yt = ys = qs = kind = 0
     if residual is not None:
-        rp, rs = _rows(residual, "residual", T, H, _FLOATS, dev)
-        rt = _FLOATS[residual.dtype]
+        rp, rt, rs = _rows(residual, "residual", shape, _FLOATS, dev)
         if residual_out is None:
             residual_out = torch.empty(T, H, dtype=residual.dtype, device=x.device)
-        rop, ros = _rows(residual_out, "residual_out", T, H, (residual.dtype,), dev)
+        rop, same, ros = _rows(residual_out, "residual_out", shape, _FLOATS, dev)
+        if same != rt:
+            raise ValueError("residual_out: needs residual's type")
     elif residual_out is not None:
         raise ValueError("residual_out without residual")
     if out is not None or dtype is not None:
         if out is None:
             out = torch.empty(T, H, dtype=dtype, device=x.device)
-        yp, ys = _rows(out, "out", T, H, _FLOATS, dev)
-        yt = _FLOATS[out.dtype]
+        yp, yt, ys = _rows(out, "out", shape, _FLOATS, dev)
     if quant is not None:
-        _need(quant in _QUANT, f"quant: one of {list(_QUANT)}")
-        kind = _QUANT[quant]
+        kind = _QUANT.get(quant)
+        if kind is None:
+            raise ValueError(f"quant: one of {list(_QUANT)}")
         n = 1 if quant == "row" else -(-H // (32 if quant == "mx" else quant))
         if q is None:
             q = torch.empty(T, H, dtype=torch.float8_e4m3fn, device=x.device)
         if q_scales is None:
             q_scales = torch.empty(T, n, dtype=torch.float8_e8m0fnu if quant == "mx" else torch.float32, device=x.device)
-        qp, qs = _rows(q, "q", T, H, _E4M3, dev)
+        qp, _, qs = _rows(q, "q", shape, _E4M3, dev)
         sp = _dense(q_scales, "q_scales", (T, n), _MX_TYPES if quant == "mx" else _F32, dev)
     elif q is not None or q_scales is not None:
         raise ValueError("q without quant")
-    _call("moe_b200_add_rmsnorm", dev, capi.AddRmsnormArgs(
-        T, H, xp, _FLOATS[x.dtype], xs, rp, rt, rs, rop, ros, wp, _FLOATS[weight.dtype], eps, yp, yt, ys, qp, qs, sp, kind))
+    _call("moe_b200_add_rmsnorm", dev, _PACK_NORM(
+        T, H, xp, xt, xs, rp, rt, rs, rop, ros, wp, _FLOATS[weight.dtype], eps, yp, yt, ys, qp, qs, sp, kind))
     return NormResult(out, residual_out, q, q_scales)
 
 
@@ -158,26 +165,26 @@ def route_logits(logits, k, *, score="softmax", bias=None, n_groups=1, topk_grou
                    group_top=group_top, renormalize=renormalize, scale=scale, counts=counts, topk_i=topk_i, topk_w=topk_w)
     dev = _device(logits)
     _need(logits.dim() == 2, "logits: needs two dimensions")
-    T, E = logits.shape
-    lp, ls = _rows(logits, "logits", T, E, _FLOATS, dev)
+    shape = logits.shape
+    T, E = shape
+    lp, lt, ls = _rows(logits, "logits", shape, _FLOATS, dev)
     _need(score in _SCORES, f"score: one of {list(_SCORES)}")
-    bp = None if bias is None else _dense(bias, "bias", (E,), _F32, dev)
+    bp = 0 if bias is None else _dense(bias, "bias", (E,), _F32, dev)
     if topk_i is None:
         topk_i = torch.empty(T, k, dtype=torch.int32, device=logits.device)
     if topk_w is None:
         topk_w = torch.empty(T, k, dtype=torch.float32, device=logits.device)
     ip = _dense(topk_i, "topk_i", (T, k), _I32, dev)
     wp = _dense(topk_w, "topk_w", (T, k), _F32, dev)
-    cp = None
+    cp = 0
     if counts is True:
         counts = torch.empty(E, dtype=torch.int32, device=logits.device)
     elif counts is False:
         counts = None
     if counts is not None:
         cp = _dense(counts, "counts", (E,), _I32, dev)
-    _call("moe_b200_route_logits", dev, capi.RouteLogitsArgs(
-        T, E, k, lp, _FLOATS[logits.dtype], ls, _SCORES[score], bp, n_groups, topk_groups, group_top, bool(renormalize), scale,
-        ip, wp, cp))
+    _call("moe_b200_route_logits", dev, _PACK_ROUTE(
+        T, E, k, lp, lt, ls, _SCORES[score], bp, n_groups, topk_groups, group_top, bool(renormalize), scale, ip, wp, cp))
     return Routing(topk_i, topk_w, counts)
 
 
@@ -198,7 +205,7 @@ def w4_matvec(x, codes, scales, bias=None, *, x_scales=None, ids=None, rows_per_
     dev = _device(x)
     _need(x.dim() == 2, "x: needs two dimensions")
     rows, K = x.shape
-    xp, xs = _rows(x, "x", rows, K, _X4, dev)
+    xp, xt, xs = _rows(x, "x", x.shape, _X4, dev)
     shape = scales.shape
     stack = len(shape) == 3
     _need(stack or len(shape) == 2, "scales: needs [N, groups] or [n, N, groups]")
@@ -207,10 +214,10 @@ def w4_matvec(x, codes, scales, bias=None, *, x_scales=None, ids=None, rows_per_
     _need(G > 0 and K % G == 0, "scales: their number must divide the columns of x")
     cp = _dense(codes, "codes", (*lead, G, 16) if codes.dim() == len(shape) + 1 else (*lead, K // 2), _U8, dev)
     sp = _dense(scales, "scales", shape, _W4_SCALES, dev)
-    bp = None if bias is None else _dense(bias, "bias", lead, _F32, dev)
+    bp = 0 if bias is None else _dense(bias, "bias", lead, _F32, dev)
     _need(rows_per_x >= 1, "rows_per_x: at least 1")
     M = rows * rows_per_x
-    ip = None
+    ip = 0
     if ids is not None:
         n = ids.numel()
         _need(M - rows_per_x < n <= M, "ids: one per row, rows_per_x for each row of x")
@@ -218,7 +225,7 @@ def w4_matvec(x, codes, scales, bias=None, *, x_scales=None, ids=None, rows_per_
         ip = _dense(ids, "ids", (M,), _I32, dev)
     else:
         _need(not stack, "a stack of matrices needs ids")
-    kind, xsp = capi.SCALE_NONE, None
+    kind, xsp = capi.SCALE_NONE, 0
     if x_scales is not None:
         _need(x_scales.dim() == 2, "x_scales: needs two dimensions")
         m = x_scales.shape[1]
@@ -235,9 +242,8 @@ def w4_matvec(x, codes, scales, bias=None, *, x_scales=None, ids=None, rows_per_
     n_out = N if swiglu is None else N // 2
     if out is None:
         out = torch.empty(M, n_out, dtype=dtype, device=x.device)
-    op, os_ = _rows(out, "out", M, n_out, _FLOATS, dev)
-    w = capi.W4Matrix(capi.W4_INT4 if scales.dtype == torch.bfloat16 else capi.W4_MXFP4, K // G, shape[0] if stack else 1, N, K,
-                      cp, sp, bp)
-    _call("moe_b200_w4_matvec", dev, capi.W4MatvecArgs(
-        w, xp, _X4[x.dtype], xs, xsp, kind, M, rows_per_x, ip, swiglu is not None, alpha, limit, op, _FLOATS[out.dtype], os_))
+    op, ot, os_ = _rows(out, "out", (M, n_out), _FLOATS, dev)
+    _call("moe_b200_w4_matvec", dev, _PACK_MATVEC(
+        capi.W4_INT4 if scales.dtype == torch.bfloat16 else capi.W4_MXFP4, K // G, shape[0] if stack else 1, N, K, cp, sp, bp,
+        xp, xt, xs, xsp, kind, M, rows_per_x, ip, swiglu is not None, alpha, limit, op, ot, os_))
     return out

@@ -1,5 +1,7 @@
 """The stand-alone operators refuse wrong arguments with a status and a text, before anything is launched:
 no GPU is needed (the pointers below are never followed)."""
+import ctypes
+
 import pytest
 import torch
 
@@ -13,14 +15,14 @@ def _norm(**kw):
     a = dict(T=4, H=64, x=A, xt=capi.DTYPE_BF16, xs=64, r=A, rt=capi.DTYPE_F32, rs=64, ro=A, ros=64, w=A, wt=capi.DTYPE_F32,
              eps=1e-5, y=A, yt=capi.DTYPE_BF16, ys=64, q=A, qs=64, sc=A, kind=capi.SCALE_ROW)
     a.update(kw)
-    return capi.lib().moe_b200_add_rmsnorm(capi.AddRmsnormArgs(*a.values()), None)
+    return capi.lib().moe_b200_add_rmsnorm(ctypes.byref(capi.AddRmsnormArgs(*a.values())), None)
 
 
 def _route(**kw):
     a = dict(T=4, E=64, K=4, l=A, dt=capi.DTYPE_F32, s=64, score=capi.SCORE_SOFTMAX, bias=None, ng=1, kg=1, gt=1, rn=1, scale=1.0,
              i=A, w=A, c=None)
     a.update(kw)
-    return capi.lib().moe_b200_route_logits(capi.RouteLogitsArgs(*a.values()), None)
+    return capi.lib().moe_b200_route_logits(ctypes.byref(capi.RouteLogitsArgs(*a.values())), None)
 
 
 def _matvec(mat=None, **kw):
@@ -29,7 +31,7 @@ def _matvec(mat=None, **kw):
     a = dict(x=A, xt=capi.DTYPE_BF16, xs=64, sc=None, kind=capi.SCALE_NONE, M=4, rpx=1, ids=None, sw=0, al=1.702, li=7.0, out=A,
              ot=capi.DTYPE_BF16, os=64)
     a.update(kw)
-    return capi.lib().moe_b200_w4_matvec(capi.W4MatvecArgs(capi.W4Matrix(**m), *a.values()), None)
+    return capi.lib().moe_b200_w4_matvec(ctypes.byref(capi.W4MatvecArgs(capi.W4Matrix(**m), *a.values())), None)
 
 
 def test_null_arguments_are_refused():
@@ -72,6 +74,30 @@ def test_route_logits_refuses(kw):
 def test_w4_matvec_refuses(mat, kw):
     assert _matvec(mat, **kw) == capi.ERR_INVALID
     assert b"w4_matvec" in capi.lib().moe_b200_last_error(None)
+
+
+def test_packed_arguments_are_the_struct():
+    for cls in (capi.AddRmsnormArgs, capi.RouteLogitsArgs, capi.W4MatvecArgs):
+        flat = []
+
+        def fill(t, at):
+            out = []
+            for _, ft in t._fields_:
+                if issubclass(ft, ctypes.Structure):
+                    out.append(fill(ft, at))
+                else:
+                    at[0] += 1
+                    v = float(at[0]) if ft is ctypes.c_float else at[0]
+                    flat.append(v)
+                    out.append(v)
+            return t(*out)
+
+        s = fill(cls, [0])
+        packed, names = capi.packer(cls)(*flat), [n for n, _ in cls._fields_]
+        back = cls.from_buffer_copy(packed)
+        for n in names:
+            a, b = getattr(s, n), getattr(back, n)
+            assert a == b if not isinstance(a, ctypes.Structure) else bytes(a)[:20] == bytes(b)[:20] and a.bias == b.bias
 
 
 def test_nothing_to_do_is_fine():
