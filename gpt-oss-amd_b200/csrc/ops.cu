@@ -169,9 +169,7 @@ moe_b200_status moe_b200_route_logits(const moe_b200_route_logits_args* args, mo
         return launched("moe_b200_route_logits: counts", cudaMemsetAsync(expert_counts, 0, sizeof(int) * (size_t)E, st));
     LogitsArgs a{logits, stride, dtype, n_tokens, E, K, score == MOE_B200_SCORE_SIGMOID, bias, n_groups, topk_groups,
                  group_top, renormalize != 0, scale, topk_i, topk_w, expert_counts};
-    // a warp per token; small batches spread over the SMs
-    const int warps = n_tokens >= 2 * ROUTE_WARPS * sms ? ROUTE_WARPS : n_tokens >= 4 * sms ? 4 : 1;
-    const int want = (n_tokens + warps - 1) / warps, most = 2 * (ROUTE_WARPS / warps) * sms;
+    const int want = (n_tokens + ROUTE_WARPS - 1) / ROUTE_WARPS, most = 8 * sms;
     const int nt = E <= 32 ? 1 : E <= 64 ? 2 : E <= 128 ? 4 : E <= 256 ? 8 : 16;
     const int piece = nt * size_of(dtype) < 16 ? nt * size_of(dtype) : 16;
     const bool vec = E % nt == 0 && rows_aligned(logits, stride, size_of(dtype), piece);
@@ -182,17 +180,23 @@ moe_b200_status moe_b200_route_logits(const moe_b200_route_logits_args* args, mo
                             : (vec ? route_logits_kernel<16, true> : route_logits_kernel<16, false>);
     const size_t per_warp = nt == 1 ? route_smem_bytes<1>() : nt == 2 ? route_smem_bytes<2>() : nt == 4 ? route_smem_bytes<4>()
                             : nt == 8 ? route_smem_bytes<8>() : route_smem_bytes<16>();
-    const size_t smem = per_warp * warps;
-    if (smem > 44 * 1024) {  // with the fixed part more than a block has without asking
-        cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)(per_warp * ROUTE_WARPS));
-        if (e != cudaSuccess)
-            return launched("moe_b200_route_logits: shared memory", e);
-    }
-    kernel<<<want < most ? want : most, 32 * warps, smem, st>>>(a);
+    static_assert(ROUTE_WARPS * (route_smem_bytes<16>() + 128) <= 48 * 1024, "what a block has without asking");
+    kernel<<<want < most ? want : most, 32 * ROUTE_WARPS, per_warp * ROUTE_WARPS, st>>>(a);
     if (expert_counts) {
+        cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess)
+            return launched("moe_b200_route_logits", e);
         const int n = n_tokens * K, blocks = (n + 2047) / 2048;
-        route_counts_kernel<<<blocks < sms ? blocks : sms, 256, 0, st>>>(topk_i, n, E, expert_counts);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = blocks < sms ? blocks : sms;
+        cfg.blockDim = 256;
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        return launched("moe_b200_route_logits: counts", cudaLaunchKernelEx(&cfg, route_counts_kernel, (const int*)topk_i, n, E, expert_counts));
     }
     return launched("moe_b200_route_logits", cudaGetLastError());
 }
