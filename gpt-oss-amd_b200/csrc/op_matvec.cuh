@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(MV_BLOCK, 2) w4_matvec_kernel(const __grid_con
             if (lane == 0)
                 mbar_expect_tx(full, rows * pieces * 16 + bulk);
             __syncwarp();
-            if (a.pitch == G * 16) {  // whole rows, as they lie
+            if (a.chunk_steps == steps) {  // whole rows, as they lie
                 if (lane == 0)
                     bulk_load(smem_u32(dyn) + 128 + l_stage * stage_bytes, a.codes + row0 * G * 16, rows * G * 16, full);
             } else if (lane < rows)

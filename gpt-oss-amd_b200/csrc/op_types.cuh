@@ -56,9 +56,9 @@ __device__ __forceinline__ void store_from_float(void* p, long long i, int dtype
         static_cast<uint16_t*>(p)[i] = (uint16_t)float_to_half(v, dtype);
 }
 
-// 2^(byte - 127) of an e8m0 byte, byte 0 included (an fp32 subnormal).  Byte 255 gives infinity.
+// 2^(byte - 127) of an e8m0 byte, byte 0 included (an fp32 subnormal).  Byte 255 is NaN.
 __device__ __forceinline__ float e8m0_to_float(uint32_t byte) {
-    return __uint_as_float(max(byte << 23, 0x00400000u));
+    return __uint_as_float(byte == 255 ? 0x7FC00000u : max(byte << 23, 0x00400000u));
 }
 
 }  // namespace op

@@ -118,12 +118,15 @@ moe_b200_status moe_b200_add_rmsnorm(const moe_b200_add_rmsnorm_args* args, moe_
                      (!residual_out || rows_aligned(residual_out, residual_out_stride, size_of(residual_dtype), 16)) &&
                      (!y || rows_aligned(y, y_stride, size_of(y_dtype), 16)) && (!q || rows_aligned(q, q_stride, 1, 8));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    const int chunks = (H + 255) / 256;  // of a warp
+    // Chunks of 256 columns per warp.  Few rows want threads, many rows registers in flight; 1, 2 and 4 chunks, us (bf16,
+    // fp32 residual, MX codes): 1 x 2880 2.5, 3.0, 5.1; 256 x 2880 3.6, 3.6, 6.0; 400 x 8192 12.4, 11.1, 14.1; 16384 x 1024 34.7,
+    // 35.8, 57.7; 16384 x 2880 97, 95, 146; 5000 x 8192 106, 83, 127.  A block has 32 warps at most.
+    const int chunks = (H + 255) / 256;
     const int nv = chunks <= 32 ? (n_rows > 2 * sms && chunks > 4 ? 2 : 1) : chunks <= 64 ? 2 : 4;
     const int threads = 32 * ((chunks + nv - 1) / nv);
     auto kernel = vec ? (nv == 1 ? add_rmsnorm_kernel<true, 1> : nv == 2 ? add_rmsnorm_kernel<true, 2> : add_rmsnorm_kernel<true, 4>)
                       : (nv == 1 ? add_rmsnorm_kernel<false, 1> : nv == 2 ? add_rmsnorm_kernel<false, 2> : add_rmsnorm_kernel<false, 4>);
-    const int together = threads == 32 && n_rows >= 8 * sms ? 8 : 1;  // rows per block
+    const int together = threads == 32 && n_rows >= 8 * sms ? 8 : 1;  // rows per block; 16384 x 64: 5.7 us, one 10.3
     kernel<<<(n_rows + together - 1) / together, dim3(threads, together), 0, st>>>(a);
     return launched("moe_b200_add_rmsnorm", cudaGetLastError());
 }
@@ -284,30 +287,38 @@ moe_b200_status moe_b200_w4_matvec(const moe_b200_w4_matvec_args* args, moe_b200
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
 
     // Pairs of x rows per pass over the weights.  Chosen matrices are shared by n_rows / n_mats rows on the average.
+    // Two pairs halve what is read, but a step has twice the MMAs and the list half the items.  One and two, us:
+    // a matrix of its own per row (32 of 2880 x 2880) 30.3, 34.5; three or four rows per matrix 5.6, 6.9 (2048 x 2880),
+    // 8.4, 9.9 (5120), 10.1, 10.1 (8192), 28.9, 26.1 (40224), 14.9, 16.0 (4 x 2880), 24.0, 23.4 (8 x 2880).
     const int share = ids ? (n_rows + w->n_mats - 1) / w->n_mats : n_rows;
-    int pairs = share <= 2 ? 1 : 2;
+    const long long shared_items = (long long)(ids ? w->n_mats : 1) * ((share + 3) / 4) * a.n_tiles;
+    int pairs = share <= 2 || shared_items < 5LL * sms ? 1 : 2;
     const int steps = mv_steps(K), sb = int4 ? 2 : 1, SG = (K / 32) >> a.group_shift;
     a.scale_slot = (MV_TILE * SG * sb + 15) / 16 * 16;
     a.scale_bulk = ((reinterpret_cast<uintptr_t>(w->scales) | (ids ? (unsigned long long)N * SG * sb : 0)) & 15) == 0;
-    // The ring: two blocks per SM where two stages of whole rows fit, else pieces of rows, else one block.
+    // The ring: rows in as few pieces as leave room for two stages in each of two blocks per SM, or for three in one.
+    // Us per 20000 rows, blocks per SM / steps of a piece / stages: 3584 columns 11.4 (2/28/2), 11.7 (2/28/3),
+    // 13.3 (1/28/4), 16.2 (2/24/3); 6144 20.5 (1/48/3), 20.9 (2/24/3), 25.4 (1/32/4); 8192 25.3 (1/64/2), 25.5 (2/32/2),
+    // 27.4 (1/32/4), 30.9 (2/16/4); 16384 44.7 (1/48/3), 45.0 (1/64/2), 53.0 (2/24/2).  Where x leaves two pairs only
+    // short pieces, two passes are faster: 4 rows, two pairs and one: 16384 columns 107 (1/16/3), 96; int4 176 (1/8/4),
+    // 105; 12288 int4 70 (1/24/3), 80.
     size_t smem = 0;
     int blocks = 0;
     for (;; pairs /= 2) {
         const size_t fixed = 1024 + mv_static_bytes(pairs);  // the system's and the kernel's own
         const size_t x_bytes = 128 + (size_t)(n_rows < 2 * pairs ? n_rows : 2 * pairs) * steps * 272;
-        for (blocks = 2; blocks >= 1 && !smem; blocks--) {
-            const size_t room = MV_SM_SMEM / blocks - fixed;
-            const int pieces[5] = {steps, 32, 24, 16, 8};  // steps of a stage: a row, or multiples of the eight warps
-            for (int i = steps <= 48 ? 0 : 1; i < 5 && !smem; i++) {
-                const int cs = pieces[i];
-                if (i > 0 && cs >= steps)
-                    continue;
-                const int pitch = cs == steps ? K / 2 : cs * 64 + 64;  // pieces of rows 64 modulo 128 apart
-                const int nc = (steps + cs - 1) / cs;
-                for (int d = MV_MAX_DEPTH; d >= 3 && !smem; d--) {
+        for (int nc = 1; nc <= (steps + MV_WARPS - 1) / MV_WARPS && !smem; nc++) {
+            const int cs = nc == 1 ? steps : ((steps + nc - 1) / nc + MV_WARPS - 1) / MV_WARPS * MV_WARPS;
+            if ((steps + cs - 1) / cs != nc)
+                continue;
+            if (pairs > 1 && nc > 1 && cs < 24)
+                break;
+            const int pitch = nc == 1 ? K / 2 : cs * 64 + 64;  // pieces of rows 64 modulo 128 apart
+            for (blocks = 2; blocks >= 1 && !smem; blocks--)
+                for (int d = MV_MAX_DEPTH; d >= (blocks == 2 ? 2 : 3) && !smem; d--) {
                     const int slots = (d - 1 + nc - 1) / nc + 1;  // tiles begun or ahead
                     const size_t need = (size_t)d * MV_TILE * pitch + (size_t)slots * a.scale_slot + x_bytes;
-                    if (need <= room) {
+                    if (need <= MV_SM_SMEM / blocks - fixed) {
                         a.depth = d;
                         a.chunk_steps = cs;
                         a.pitch = pitch;
@@ -315,7 +326,6 @@ moe_b200_status moe_b200_w4_matvec(const moe_b200_w4_matvec_args* args, moe_b200
                         smem = need;
                     }
                 }
-            }
         }
         blocks++;
         if (smem || pairs == 1)

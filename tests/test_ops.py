@@ -431,6 +431,52 @@ def test_w4_matvec_every_scale_byte():
     assert (pkg.w4_matvec(torch.ones(1, K, dtype=BF16, device="cuda"), codes, scales, dtype=F32)[0, :255] == 0).all()
 
 
+@pytest.mark.parametrize("N,K,M,fmt,group,kind", [
+    # two pairs of rows per pass: many tiles, or many rows
+    (12000, 160, 3, "mxfp4", 32, BF16), (12001, 2880, 4, "int4", 32, "mx"), (320, 4096, 255, "mxfp4", 32, F16),
+    (12003, 8192, 4, "mxfp4", 32, "row"), (12007, 12288, 3, "int4", 64, BF16), (12010, 16384, 4, "int4", 128, 128),
+    # one, rows whole and in pieces
+    (300, 5760, 1, "mxfp4", 32, BF16), (300, 6144, 2, "int4", 128, 64), (299, 8192, 1, "mxfp4", 32, F16),
+    (301, 11264, 2, "int4", 32, "mx"), (303, 11296, 1, "mxfp4", 32, BF16), (300, 16384, 1, "mxfp4", 32, "row"),
+    (5003, 4096, 1, "mxfp4", 32, BF16), (5000, 16352, 1, "int4", 32, BF16)])
+def test_w4_matvec_rings(N, K, M, fmt, group, kind):
+    """Each way to divide shared memory among x, stages and blocks."""
+    g = _gen(N + K + M)
+    codes, scales = _weights(g, (), N, K, fmt, group)
+    b = 0.1 * _randn(g, N)
+    x, xsc, x64 = _x(g, M, K, kind)
+    y = pkg.w4_matvec(x, codes, scales, b, x_scales=xsc, dtype=F32)
+    _check_matvec(y, x64, codes, scales, b, group, None, 1)
+
+
+def test_w4_matvec_one_and_two_pairs_agree():
+    """The same bits alone and in a batch that passes over the weights with two pairs of rows."""
+    g = _gen(5)
+    n, N, K = 4, 3000, 544
+    codes, scales = _weights(g, (n,), N, K, "int4", 32)
+    x, _, x64 = _x(g, 16, K, BF16)
+    ids = torch.tensor([0, 1, 2, 3, 3, 2, 1, 0, 0, 0, 1, 1, 2, 2, 3, 3], dtype=torch.int32, device="cuda")
+    y = pkg.w4_matvec(x, codes, scales, ids=ids, dtype=F32)
+    _check_matvec(y, x64, codes, scales, None, 32, ids, 1)
+    for m in range(16):
+        assert torch.equal(y[m:m + 1], pkg.w4_matvec(x[m:m + 1], codes, scales, ids=ids[m:m + 1], dtype=F32))
+
+
+def test_w4_matvec_x_scale_bytes():
+    """The e8m0 scales of x: 2^(byte - 127), 255 is NaN and stays in its row."""
+    K = 32
+    codes = torch.zeros(16, K // 2, dtype=torch.uint8, device="cuda")
+    codes[:, 0] = 0x02  # 1.0 in column 0
+    scales = torch.full((16, 1), 127, dtype=torch.uint8, device="cuda")
+    x = torch.zeros(256, K, device="cuda")
+    x[:, 0] = 1.0
+    x = x.to(torch.float8_e4m3fn)
+    sx = torch.arange(256, device="cuda").to(torch.uint8).view(256, 1)
+    y = pkg.w4_matvec(x, codes, scales, x_scales=sx, dtype=F32).double()
+    assert y[255].isnan().all()
+    assert torch.equal(y[:255], (torch.arange(255, device="cuda").double() - 127).exp2()[:, None].expand(255, 16))
+
+
 @pytest.mark.parametrize("mag", [1e-30, 1e-6, 1.0, 1e6, 1e30])
 def test_w4_matvec_bf16_of_any_size(mag):
     """bf16 x far outside fp16's range, groups of very different size in one row."""
