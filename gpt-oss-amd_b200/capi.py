@@ -18,6 +18,7 @@ DTYPE_F32, DTYPE_BF16, DTYPE_F16, DTYPE_E4M3 = range(4)
 SCALE_NONE, SCALE_ROW, SCALE_G32, SCALE_G64, SCALE_G128, SCALE_MX = range(6)
 SCORE_SOFTMAX, SCORE_SIGMOID = range(2)
 W4_MXFP4, W4_INT4 = range(2)
+W4_MATVEC_MAX_ROWS = 256
 GEMM_TCGEN05 = 0
 GEMM_MMA_SYNC = 1  # exists in the test-aids build only
 EP_PEER_EXPORT_BYTES = 256
@@ -67,7 +68,14 @@ def packer(*structs):
 
     p = struct.Struct("@" + "".join(fmt(s) for s in structs) + "0q")  # padded to its alignment
     assert p.size == sum(ctypes.sizeof(s) for s in structs)
-    return p.pack
+
+    def pack(*values):
+        try:
+            return p.pack(*values)
+        except struct.error as e:
+            raise ValueError(f"an argument does not fit the C interface: {e}") from None
+
+    return pack
 
 
 _i, _f, _p, _ll = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_longlong

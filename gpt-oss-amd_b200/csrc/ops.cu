@@ -57,9 +57,9 @@ bool is_float_type(int dtype) {
 
 bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-// Rows of `stride` elements of `size` bytes on `n`-byte boundaries.
-bool rows_aligned(const void* p, long long stride, int size, size_t n) {
-    return aligned(p, n) && ((unsigned long long)stride * (unsigned)size) % n == 0;
+// `rows` rows, `stride` elements of `size` bytes apart, on `n`-byte boundaries.
+bool rows_aligned(const void* p, int rows, long long stride, int size, size_t n) {
+    return aligned(p, n) && (rows <= 1 || ((unsigned long long)stride * (unsigned)size) % n == 0);
 }
 
 }  // namespace
@@ -113,10 +113,10 @@ moe_b200_status moe_b200_add_rmsnorm(const moe_b200_add_rmsnorm_args* args, moe_
     NormArgs a{x, x_stride, x_dtype, residual, residual_out, residual_stride, residual_out_stride, residual_dtype,
                weight, weight_dtype, eps, n_rows, H, y, y_stride, y_dtype, static_cast<uint8_t*>(q), q_stride, q_scales,
                n_scales, group, group == 128 ? 7 : group == 64 ? 6 : 5, mx};
-    const bool vec = H % 8 == 0 && rows_aligned(x, x_stride, size_of(x_dtype), 16) && aligned(weight, 16) &&
-                     (!residual || rows_aligned(residual, residual_stride, size_of(residual_dtype), 16)) &&
-                     (!residual_out || rows_aligned(residual_out, residual_out_stride, size_of(residual_dtype), 16)) &&
-                     (!y || rows_aligned(y, y_stride, size_of(y_dtype), 16)) && (!q || rows_aligned(q, q_stride, 1, 8));
+    const bool vec = H % 8 == 0 && rows_aligned(x, n_rows, x_stride, size_of(x_dtype), 16) && aligned(weight, 16) &&
+                     (!residual || rows_aligned(residual, n_rows, residual_stride, size_of(residual_dtype), 16)) &&
+                     (!residual_out || rows_aligned(residual_out, n_rows, residual_out_stride, size_of(residual_dtype), 16)) &&
+                     (!y || rows_aligned(y, n_rows, y_stride, size_of(y_dtype), 16)) && (!q || rows_aligned(q, n_rows, q_stride, 1, 8));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     // Chunks of 256 columns per warp.  Few rows want threads, many rows registers in flight; 1, 2 and 4 chunks, us (bf16,
     // fp32 residual, MX codes): 1 x 2880 2.5, 3.0, 5.1; 256 x 2880 3.6, 3.6, 6.0; 400 x 8192 12.4, 11.1, 14.1; 16384 x 1024 34.7,
@@ -127,7 +127,7 @@ moe_b200_status moe_b200_add_rmsnorm(const moe_b200_add_rmsnorm_args* args, moe_
     auto kernel = vec ? (nv == 1 ? add_rmsnorm_kernel<true, 1> : nv == 2 ? add_rmsnorm_kernel<true, 2> : add_rmsnorm_kernel<true, 4>)
                       : (nv == 1 ? add_rmsnorm_kernel<false, 1> : nv == 2 ? add_rmsnorm_kernel<false, 2> : add_rmsnorm_kernel<false, 4>);
     const int together = threads == 32 && n_rows >= 8 * sms ? 8 : 1;  // rows per block; 16384 x 64: 5.7 us, one 10.3
-    kernel<<<(n_rows + together - 1) / together, dim3(threads, together), 0, st>>>(a);
+    kernel<<<(unsigned)(((long long)n_rows + together - 1) / together), dim3(threads, together), 0, st>>>(a);
     return launched("moe_b200_add_rmsnorm", cudaGetLastError());
 }
 
@@ -175,7 +175,7 @@ moe_b200_status moe_b200_route_logits(const moe_b200_route_logits_args* args, mo
     const int want = (n_tokens + ROUTE_WARPS - 1) / ROUTE_WARPS, most = 8 * sms;
     const int nt = E <= 32 ? 1 : E <= 64 ? 2 : E <= 128 ? 4 : E <= 256 ? 8 : 16;
     const int piece = nt * size_of(dtype) < 16 ? nt * size_of(dtype) : 16;
-    const bool vec = E % nt == 0 && rows_aligned(logits, stride, size_of(dtype), piece);
+    const bool vec = E % nt == 0 && rows_aligned(logits, n_tokens, stride, size_of(dtype), piece);
     auto kernel = nt == 1 ? (vec ? route_logits_kernel<1, true> : route_logits_kernel<1, false>)
                   : nt == 2 ? (vec ? route_logits_kernel<2, true> : route_logits_kernel<2, false>)
                   : nt == 4 ? (vec ? route_logits_kernel<4, true> : route_logits_kernel<4, false>)
@@ -251,7 +251,7 @@ moe_b200_status moe_b200_w4_matvec(const moe_b200_w4_matvec_args* args, moe_b200
     const int n_out = swiglu ? N / 2 : N;
     if (x_stride < 0 || (n_rows > 1 && out_stride < n_out))
         INVALID("moe_b200_w4_matvec: x_stride is not negative, rows of out do not overlap");
-    if (!aligned(w->codes, 16) || !rows_aligned(x, x_stride, size_of(x_dtype), x_dtype == MOE_B200_DTYPE_E4M3 ? 8 : 16))
+    if (!aligned(w->codes, 16) || !rows_aligned(x, (n_rows - 1) / rows_per_x + 1, x_stride, size_of(x_dtype), x_dtype == MOE_B200_DTYPE_E4M3 ? 8 : 16))
         INVALID("moe_b200_w4_matvec: codes and rows of x must be 16-byte aligned (rows of e4m3 8-byte aligned)");
     if ((int4 && !aligned(w->scales, 2)) || !aligned(w->bias, 4) || !aligned(ids, 4) || !aligned(out, size_of(out_dtype)) ||
         (n_xs && x_scale_kind != MOE_B200_SCALE_MX && !aligned(x_scales, 4)))

@@ -78,10 +78,11 @@ def _device(t):
     return dev
 
 
-def _on(stream, fn, *args, **kw):
+def _on(stream, fn, x, *args, **kw):
     """The call with `stream` as the current one: new results come from that stream's memory."""
+    _need(stream.device == x.device, "stream: needs the device of the tensors")
     with torch.cuda.stream(stream):
-        return fn(*args, **kw)
+        return fn(x, *args, **kw)
 
 
 def _call(name, dev, args):
@@ -168,6 +169,7 @@ def route_logits(logits, k, *, score="softmax", bias=None, n_groups=1, topk_grou
     shape = logits.shape
     T, E = shape
     lp, lt, ls = _rows(logits, "logits", shape, _FLOATS, dev)
+    _need(1 <= k <= E, "k: needs 1 to the number of experts")
     _need(score in _SCORES, f"score: one of {list(_SCORES)}")
     bp = 0 if bias is None else _dense(bias, "bias", (E,), _F32, dev)
     if topk_i is None:
@@ -238,6 +240,7 @@ def w4_matvec(x, codes, scales, bias=None, *, x_scales=None, ids=None, rows_per_
             _need(len(fits) == 1, "x_scales: one per row or per 32, 64 or 128 columns")
             kind, want = _QUANT[fits[0]], m
         xsp = _dense(x_scales, "x_scales", (rows, want), _X_SCALES, dev)
+    _need(M <= capi.W4_MATVEC_MAX_ROWS, "w4_matvec: at most 256 rows (larger batches are matrix products)")
     alpha, limit = swiglu if swiglu is not None else (0.0, 0.0)
     n_out = N if swiglu is None else N // 2
     if out is None:

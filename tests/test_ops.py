@@ -533,6 +533,58 @@ def test_w4_matvec_a_row_does_not_depend_on_the_batch():
         assert torch.equal(y[m:m + 1], pkg.w4_matvec(x[m:m + 1], codes[int(ids[m])], scales[int(ids[m])], dtype=F32))
 
 
+def test_wrappers_refuse_on_the_device():
+    """What the CPU cannot show behind its own refusal: shapes, types and ranges of CUDA tensors, before any launch."""
+    from types import SimpleNamespace
+
+    x = torch.zeros(4, 64, dtype=BF16, device="cuda")
+    w, res = torch.ones(64, device="cuda"), torch.zeros(4, 64, device="cuda")
+    codes, scales = torch.zeros(8, 32, dtype=torch.uint8, device="cuda"), torch.zeros(8, 2, dtype=torch.uint8, device="cuda")
+    q = torch.zeros(4, 64, dtype=torch.float8_e4m3fn, device="cuda")
+    ids = torch.zeros(4, dtype=torch.int32, device="cuda")
+    wide = torch.zeros(4, 67, dtype=BF16, device="cuda")[:, :64]
+    elsewhere = SimpleNamespace(device=torch.device("cuda", torch.cuda.device_count()))
+    for call in [
+        lambda: pkg.add_rmsnorm(x[0], w), lambda: pkg.add_rmsnorm(x.double(), w), lambda: pkg.add_rmsnorm(x.t(), w),
+        lambda: pkg.add_rmsnorm(x, w[:63]), lambda: pkg.add_rmsnorm(x, w.cpu()), lambda: pkg.add_rmsnorm(x, w, res[:3]),
+        lambda: pkg.add_rmsnorm(x, w, residual_out=x), lambda: pkg.add_rmsnorm(x, w, x, residual_out=res),
+        lambda: pkg.add_rmsnorm(x, w, quant=16), lambda: pkg.add_rmsnorm(x, w, q=q), lambda: pkg.add_rmsnorm(x, w, dtype=torch.int8),
+        lambda: pkg.add_rmsnorm(x, w, quant="mx", q_scales=torch.zeros(4, 2, device="cuda")),
+        lambda: pkg.add_rmsnorm(x, w, eps=1e300), lambda: pkg.add_rmsnorm(x, w, eps=-1.0), lambda: pkg.add_rmsnorm(x, w, dtype=None),
+        lambda: pkg.add_rmsnorm(x[:1].expand(4, 64), w, out=x[:1].expand(4, 64)), lambda: pkg.add_rmsnorm(x, w, stream=elsewhere),
+        lambda: pkg.route_logits(x[0], 4), lambda: pkg.route_logits(x, 0), lambda: pkg.route_logits(x, -1),
+        lambda: pkg.route_logits(x, 65), lambda: pkg.route_logits(x, 17), lambda: pkg.route_logits(x, 4, score="max"),
+        lambda: pkg.route_logits(x, 4, bias=w[:63]), lambda: pkg.route_logits(x, 4, topk_i=torch.zeros(4, 4, device="cuda")),
+        lambda: pkg.route_logits(x, 4, n_groups=3), lambda: pkg.route_logits(x, 4, n_groups=2**40),
+        lambda: pkg.route_logits(x, 4, scale=math.inf), lambda: pkg.route_logits(x, 4, stream=elsewhere),
+        lambda: pkg.w4_matvec(x.float(), codes, scales), lambda: pkg.w4_matvec(x, codes[:, :31], scales),
+        lambda: pkg.w4_matvec(x, codes, scales[:7]), lambda: pkg.w4_matvec(x, codes, scales.float()),
+        lambda: pkg.w4_matvec(x, codes[None], scales[None]), lambda: pkg.w4_matvec(x, codes, scales, ids=ids.long()),
+        lambda: pkg.w4_matvec(x, codes[None], scales[None], ids=ids[:0]), lambda: pkg.w4_matvec(q, codes, scales),
+        lambda: pkg.w4_matvec(q, codes, scales, x_scales=torch.zeros(4, 5, device="cuda")), lambda: pkg.w4_matvec(wide, codes, scales),
+        lambda: pkg.w4_matvec(x, codes, scales, x_scales=torch.zeros(4, 1, device="cuda")),
+        lambda: pkg.w4_matvec(x, codes, scales, rows_per_x=0), lambda: pkg.w4_matvec(x, codes, scales, rows_per_x=65),
+        lambda: pkg.w4_matvec(x, codes, scales, rows_per_x=2**40), lambda: pkg.w4_matvec(x, codes, scales, out=torch.zeros(4, 7, device="cuda")),
+        lambda: pkg.w4_matvec(x, codes, scales, swiglu=(1.7, -1.0)), lambda: pkg.w4_matvec(x, codes, scales, stream=elsewhere),
+    ]:
+        with pytest.raises((ValueError, pkg.capi.MoEError)):
+            call()
+
+
+def test_one_row_of_any_stride():
+    """The stride of a single row means nothing: rows cut out of odd buffers."""
+    g = _gen(3)
+    codes, scales = _weights(g, (), 40, 64, "mxfp4", 32)
+    wide = _randn(g, 3, 67).to(BF16)
+    x = wide[:1, :64]
+    assert torch.equal(pkg.w4_matvec(x, codes, scales, rows_per_x=3), pkg.w4_matvec(x.contiguous(), codes, scales, rows_per_x=3))
+    w = _randn(g, 64)
+    for a, b in zip(pkg.add_rmsnorm(x, w, x, quant="mx"), pkg.add_rmsnorm(x.contiguous(), w, x.contiguous(), quant="mx")):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    for a, b in zip(pkg.route_logits(x, 5)[:2], pkg.route_logits(x.contiguous(), 5)[:2]):
+        assert torch.equal(a, b)
+
+
 # -- streams, graphs, the run of them together -------------------------------------
 
 

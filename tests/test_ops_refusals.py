@@ -161,3 +161,20 @@ def test_python_wrappers_refuse():
     ]:
         with pytest.raises(ValueError):
             call()
+
+
+def test_numbers_that_do_not_fit_the_structs():
+    pack, n = capi.packer(capi.RouteLogitsArgs), len(capi.RouteLogitsArgs._fields_)
+
+    def with_value(at, v):
+        values = [0] * n
+        values[at] = v
+        return pack(*values)
+
+    for at, v in [(0, 2**31), (1, -2**31 - 1), (5, 2**63), (2, 1.5)]:
+        with pytest.raises(ValueError):
+            with_value(at, v)
+    # a float too large becomes infinity, as in C, which the library refuses
+    assert capi.RouteLogitsArgs.from_buffer_copy(with_value(12, 1e300)).scale == float("inf")
+    assert _route(scale=float("inf")) == capi.ERR_INVALID
+    assert _norm(eps=float("inf")) == capi.ERR_INVALID
