@@ -33,6 +33,7 @@
 // decodes in 9 operations per 8 codes instead of 7: 83 us; a second pair of x rows adds 8 MMAs and
 // their x to a step: 104 us.  Four pairs per pass were slower than two passes (230 against 2 x 88 us).
 #pragma once
+#include "common.cuh"
 #include "op_types.cuh"
 #include "tc5_ptx.cuh"
 
@@ -248,6 +249,9 @@ __global__ void __launch_bounds__(MV_BLOCK, 2) w4_matvec_kernel(const __grid_con
         s_abort = 0;
         fence_barrier_init();
     }
+
+    pdl_wait();
+    pdl_trigger();
 
     // the list of leaders: rows that open a pass over their matrix
     int n_lead;

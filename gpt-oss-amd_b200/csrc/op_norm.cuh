@@ -5,7 +5,7 @@
 // from the same registers, so a row is read once and written once: 2 H (read) + 8 H + 2 H + H bytes
 // for a bf16 x, an fp32 residual, a bf16 y and codes.  For many rows HBM bounds it (16384 x 2880 in bf16,
 // fp32 residual, y, codes and row scales, 613 MB: 96 us, 6.4 TB/s), for one row the chain load -> sum over the
-// block -> store (2.3 us, launch included).
+// block -> store (2.0 us, launch included).
 //
 // A block owns a row (a warp, where a warp holds it and there are many) and a thread 8 * NV columns of it in
 // registers.  VEC: eight neighbouring columns per step, moved 16 bytes at a time (rows on 16-byte boundaries, H a
@@ -15,6 +15,7 @@
 // Scales.  A group's largest |y| is found among its own lanes (a group is 4, 8 or 16 lanes with
 // VEC, one, two or four steps of a warp without), a row's over the block.
 #pragma once
+#include "common.cuh"
 #include "op_types.cuh"
 
 namespace moe {
@@ -42,6 +43,7 @@ struct NormArgs {
     int group;      // columns per scale: 32, 64, 128; 0: the row
     int group_shift;
     int mx;         // e8m0 scales
+    int early;      // the next kernel's blocks may come at once
 };
 
 // Eight values of one thread, still as they were loaded.
@@ -181,6 +183,9 @@ __device__ __forceinline__ float norm_put_scale(const NormArgs& a, long long i, 
 template <bool VEC, int NV>
 __global__ void __launch_bounds__(1024) add_rmsnorm_kernel(const NormArgs a) {
     __shared__ float slots[64];
+    pdl_wait();
+    if (a.early)
+        pdl_trigger();
     const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;  // blockDim.y > 1: a warp per row
     if (row >= a.n_rows)
         return;

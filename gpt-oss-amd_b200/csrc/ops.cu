@@ -47,6 +47,26 @@ moe_b200_status current_device(int* dev, int* sms) {
     return MOE_B200_OK;
 }
 
+// Launches as a programmatic dependent of the kernel in front: every kernel here waits for its end before it touches
+// global memory, and then lets the next one's blocks come to the SMs (`early`) if it has two blocks per SM at most.
+// Behind larger grids they would crowd where room is first: us per call in a replayed chain, launched the ordinary way,
+// always early, by this rule: add_rmsnorm 1 x 2880 2.2, 2.0, 2.0; 777 x 2047 6.4, 7.6, 6.3; route_logits 1 x 128 2.7, 2.2,
+// 2.2; 3001 x 60 3.6, 3.8, 3.2; w4_matvec 5120 x 2880 6.4, 5.7, 5.7.
+template <typename... Params, typename... Args>
+cudaError_t launch(void (*kernel)(Params...), unsigned grid, dim3 block, size_t smem, cudaStream_t stream, const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 moe_b200_status launched(const char* what, cudaError_t e) {
     return e == cudaSuccess ? MOE_B200_OK : refuse(MOE_B200_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
@@ -112,7 +132,7 @@ moe_b200_status moe_b200_add_rmsnorm(const moe_b200_add_rmsnorm_args* args, moe_
         return st;
     NormArgs a{x, x_stride, x_dtype, residual, residual_out, residual_stride, residual_out_stride, residual_dtype,
                weight, weight_dtype, eps, n_rows, H, y, y_stride, y_dtype, static_cast<uint8_t*>(q), q_stride, q_scales,
-               n_scales, group, group == 128 ? 7 : group == 64 ? 6 : 5, mx};
+               n_scales, group, group == 128 ? 7 : group == 64 ? 6 : 5, mx, 0};
     const bool vec = H % 8 == 0 && rows_aligned(x, n_rows, x_stride, size_of(x_dtype), 16) && aligned(weight, 16) &&
                      (!residual || rows_aligned(residual, n_rows, residual_stride, size_of(residual_dtype), 16)) &&
                      (!residual_out || rows_aligned(residual_out, n_rows, residual_out_stride, size_of(residual_dtype), 16)) &&
@@ -127,8 +147,9 @@ moe_b200_status moe_b200_add_rmsnorm(const moe_b200_add_rmsnorm_args* args, moe_
     auto kernel = vec ? (nv == 1 ? add_rmsnorm_kernel<true, 1> : nv == 2 ? add_rmsnorm_kernel<true, 2> : add_rmsnorm_kernel<true, 4>)
                       : (nv == 1 ? add_rmsnorm_kernel<false, 1> : nv == 2 ? add_rmsnorm_kernel<false, 2> : add_rmsnorm_kernel<false, 4>);
     const int together = threads == 32 && n_rows >= 8 * sms ? 8 : 1;  // rows per block; 16384 x 64: 5.7 us, one 10.3
-    kernel<<<(unsigned)(((long long)n_rows + together - 1) / together), dim3(threads, together), 0, st>>>(a);
-    return launched("moe_b200_add_rmsnorm", cudaGetLastError());
+    const unsigned grid = (unsigned)(((long long)n_rows + together - 1) / together);
+    a.early = grid <= 2u * sms;
+    return launched("moe_b200_add_rmsnorm", launch(kernel, grid, dim3(threads, together), 0, st, a));
 }
 
 moe_b200_status moe_b200_route_logits(const moe_b200_route_logits_args* args, moe_b200_stream stream) {
@@ -171,7 +192,7 @@ moe_b200_status moe_b200_route_logits(const moe_b200_route_logits_args* args, mo
     if (n_tokens == 0)
         return launched("moe_b200_route_logits: counts", cudaMemsetAsync(expert_counts, 0, sizeof(int) * (size_t)E, st));
     LogitsArgs a{logits, stride, dtype, n_tokens, E, K, score == MOE_B200_SCORE_SIGMOID, bias, n_groups, topk_groups,
-                 group_top, renormalize != 0, scale, topk_i, topk_w, expert_counts};
+                 group_top, renormalize != 0, scale, topk_i, topk_w, expert_counts, 0};
     const int want = (n_tokens + ROUTE_WARPS - 1) / ROUTE_WARPS, most = 8 * sms;
     const int nt = E <= 32 ? 1 : E <= 64 ? 2 : E <= 128 ? 4 : E <= 256 ? 8 : 16;
     const int piece = nt * size_of(dtype) < 16 ? nt * size_of(dtype) : 16;
@@ -184,24 +205,14 @@ moe_b200_status moe_b200_route_logits(const moe_b200_route_logits_args* args, mo
     const size_t per_warp = nt == 1 ? route_smem_bytes<1>() : nt == 2 ? route_smem_bytes<2>() : nt == 4 ? route_smem_bytes<4>()
                             : nt == 8 ? route_smem_bytes<8>() : route_smem_bytes<16>();
     static_assert(ROUTE_WARPS * (route_smem_bytes<16>() + 128) <= 48 * 1024, "what a block has without asking");
-    kernel<<<want < most ? want : most, 32 * ROUTE_WARPS, per_warp * ROUTE_WARPS, st>>>(a);
-    if (expert_counts) {
-        cudaError_t e = cudaGetLastError();
-        if (e != cudaSuccess)
-            return launched("moe_b200_route_logits", e);
+    const int grid = want < most ? want : most;
+    a.early = expert_counts || grid <= 2 * sms;  // counts: by a small grid
+    cudaError_t e = launch(kernel, grid, 32 * ROUTE_WARPS, per_warp * ROUTE_WARPS, st, a);
+    if (e == cudaSuccess && expert_counts) {
         const int n = n_tokens * K, blocks = (n + 2047) / 2048;
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = blocks < sms ? blocks : sms;
-        cfg.blockDim = 256;
-        cfg.stream = st;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        return launched("moe_b200_route_logits: counts", cudaLaunchKernelEx(&cfg, route_counts_kernel, (const int*)topk_i, n, E, expert_counts));
+        e = launch(route_counts_kernel, blocks < sms ? blocks : sms, 256, 0, st, (const int*)topk_i, n, E, expert_counts);
     }
-    return launched("moe_b200_route_logits", cudaGetLastError());
+    return launched("moe_b200_route_logits", e);
 }
 
 moe_b200_status moe_b200_w4_matvec(const moe_b200_w4_matvec_args* args, moe_b200_stream stream) {
@@ -348,8 +359,7 @@ moe_b200_status moe_b200_w4_matvec(const moe_b200_w4_matvec_args* args, moe_b200
     }
     const long long passes = ids ? n_rows : (n_rows + 2 * pairs - 1) / (2 * pairs);
     const long long items = passes * a.n_tiles, most = (long long)blocks * sms;
-    kernel<<<(unsigned)(items < most ? items : most), MV_BLOCK, smem, st>>>(a);
-    return launched("moe_b200_w4_matvec", cudaGetLastError());
+    return launched("moe_b200_w4_matvec", launch(kernel, (unsigned)(items < most ? items : most), MV_BLOCK, smem, st, a));
 }
 
 }  // extern "C"

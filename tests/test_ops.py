@@ -640,6 +640,45 @@ def test_token_step_in_8_bits_follows_the_64_bit_formulas():
     _check_matvec(h, x64, p["c1"].flatten(-2), p["s1"], p["b1"], 32, ids, 4, (1.702, 7.0))
 
 
+@pytest.mark.parametrize("T", [1, 3, 300])
+def test_long_chain_without_waits_between(T):
+    """Each call reads what the one or two in front wrote and overwrites what they read: the same bits as with the
+    device idle between the calls, eagerly and replayed."""
+    g = _gen(T)
+    H, E, K, M = 256, 16, 4, min(T, 64)
+    w = 1 + 0.1 * _randn(g, H)
+    codes, scales = _weights(g, (E,), H, H, "mxfp4", 32)
+    start = _randn(g, T, H)
+    x, res, y = (torch.empty(T, H, device="cuda", dtype=d) for d in (F32, F32, BF16))
+    q, qs = torch.empty(T, H, dtype=torch.float8_e4m3fn, device="cuda"), torch.empty(T, H // 32, dtype=torch.uint8, device="cuda")
+    ti, tw = torch.empty(T, K, dtype=torch.int32, device="cuda"), torch.empty(T, K, device="cuda")
+    counts = torch.empty(E, dtype=torch.int32, device="cuda")
+    seen = torch.empty(20, E, dtype=torch.int32, device="cuda")
+
+    def chain(pause=lambda: None):
+        x.copy_(start)
+        res.zero_()
+        for i in range(20):
+            pkg.add_rmsnorm(x, w, res, residual_out=res, out=y, quant="mx", q=q, q_scales=qs)
+            pause()
+            pkg.route_logits(y[:, :E], K, counts=counts, topk_i=ti, topk_w=tw)
+            pause()
+            pkg.w4_matvec(q[:M], codes, scales, x_scales=qs[:M], ids=ti[:M, i % K].contiguous() if i % 2 else ti.view(-1)[:M], out=x[:M])
+            pause()
+            seen[i].copy_(counts)
+        return [t.clone() for t in (x, res, y, ti, tw, seen)]
+
+    want = chain(torch.cuda.synchronize)
+    assert all(torch.equal(a, b) for a, b in zip(chain(), want))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain()
+    for _ in range(3):
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_other_streams_and_overlapping_calls():
     """Calls on streams of their own at the same time give what they give one after the other."""
     shape = pkg.MoEShape(hidden=576, intermediate=320, n_experts=32, top_k=4)
