@@ -394,7 +394,9 @@ moe_b200_status moe_b200_route_noalloc(const void* t, int t_dtype, int n_tokens,
  * allocation, nothing kept between calls: calls may overlap on any streams and
  * host threads and may be captured into graphs.  Device pointers and a stream of
  * the current device.  Strides are in elements between two rows.  Nothing outside
- * the stated rows and columns is written. */
+ * the stated rows and columns is written.  The kernels wait for all work in front of
+ * them; a kernel that the caller launches behind one as its programmatic dependent has
+ * to wait too (griddepcontrol.wait) before it touches their tensors. */
 
 /* Scales of 8-bit rows: none, one fp32 per row, one fp32 per group of 32 / 64 /
  * 128 neighbouring columns (the last group may be shorter), one e8m0 byte per
