@@ -11,8 +11,10 @@
 // 64-bit keys, a few tokens in a thousand for fp32 logits; where it hung on the groups, or on more
 // than 32 experts, it does the token again in 64 bits (route_exact).
 //
-// A warp owns a token; lane i holds the NT neighbouring experts from i * NT on, so the lowest
-// lane of a tie has the lowest index.  Each lane puts its keys in order once, by counting for each
+// A warp owns a token; a lane holds NT neighbouring experts, lanes and experts in the same order, so the
+// lowest lane of a tie has the lowest index.  Where NT allows it every group has 2^n lanes of its own, the last
+// of them empty if need be, and is scored and dropped by lanes (240 experts in 4 groups, 4096 tokens: 11.6 us
+// without, 7.8 with).  Each lane puts its keys in order once, by counting for each
 // the keys in front of it; then a round per selected expert takes the largest of the 32 heads (one
 // warp reduction) and the winner moves on to its next key.  The logits are read once, 16 bytes a
 // lane where they are aligned.
@@ -44,6 +46,7 @@ struct LogitsArgs {
     int sigmoid;
     const float* bias;
     int n_groups, topk_groups, group_top;
+    int lane_shift, lane_groups, lane_size;  // 2^lane_shift lanes for each of lane_groups groups of lane_size experts
     int renorm;
     float scale;
     int* topk_i;
@@ -206,13 +209,15 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, NT == 16 ? 5 : 8) route_logi
     // Without a bias the logits are the keys of the experts, and of groups that are scored by their best.
     const bool by_logit = a.bias == nullptr;
     const bool need_p = !by_logit || (a.n_groups > 1 && a.group_top > 1);
-    const int gs = a.E / a.n_groups, span = gs / NT;  // lanes of a group, where that is a power of two of them
-    const bool lanes_of_group = gs % NT == 0 && (span & (span - 1)) == 0;
+    const int gs = a.E / a.n_groups, span = 1 << a.lane_shift;
+    const bool lanes_of_group = a.lane_groups == a.n_groups;
+    // this lane's experts: `have` from e0 on
+    const int in_group = (lane & (span - 1)) * NT, e0 = (lane >> a.lane_shift) * a.lane_size + in_group;
+    const int have = lane >> a.lane_shift < a.lane_groups ? min(max(a.lane_size - in_group, 0), NT) : 0;
     float bias[NT];
 #pragma unroll
     for (int j = 0; j < NT; j++) {
-        const int e = lane * NT + j;
-        const float b = a.bias && e < a.E ? a.bias[e] : 0.f;
+        const float b = a.bias && j < have ? a.bias[e0 + j] : 0.f;
         bias[j] = b > -INFINITY ? fminf(b, FLT_MAX) : -INFINITY;
     }
     sorted[NT][lane] = make_float2(-INFINITY, 0.f);
@@ -220,9 +225,9 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, NT == 16 ? 5 : 8) route_logi
     for (int t = blockIdx.x * ROUTE_WARPS + warp; t < a.T; t += gridDim.x * ROUTE_WARPS) {
         float l[NT];
         const long long at = (long long)t * a.stride;
-        if (VEC && lane * NT + NT <= a.E) {
+        if (VEC && have == NT) {
             if (a.dtype == MOE_B200_DTYPE_F32) {
-                const float* src = static_cast<const float*>(a.logits) + at + lane * NT;
+                const float* src = static_cast<const float*>(a.logits) + at + e0;
                 if (NT >= 4) {
 #pragma unroll
                     for (int j = 0; j < NT; j += 4) {
@@ -235,7 +240,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, NT == 16 ? 5 : 8) route_logi
                         l[j] = src[j];
                 }
             } else {
-                const uint16_t* src = static_cast<const uint16_t*>(a.logits) + at + lane * NT;
+                const uint16_t* src = static_cast<const uint16_t*>(a.logits) + at + e0;
                 uint32_t w[(NT + 1) / 2];
                 if (NT >= 8) {
 #pragma unroll
@@ -257,10 +262,8 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, NT == 16 ? 5 : 8) route_logi
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < NT; j++) {
-                const int e = lane * NT + j;
-                l[j] = e < a.E ? load_as_float(a.logits, at + e, a.dtype) : -INFINITY;
-            }
+            for (int j = 0; j < NT; j++)
+                l[j] = j < have ? load_as_float(a.logits, at + e0 + j, a.dtype) : -INFINITY;
         }
         float lmax = -INFINITY;
 #pragma unroll
@@ -315,7 +318,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, NT == 16 ? 5 : 8) route_logi
                 if (!lanes_of_group) {
 #pragma unroll
                     for (int j = 0; j < NT; j++)
-                        s_keys[lane * NT + j] = l[j] > -INFINITY ? key[j] : -INFINITY;
+                        s_keys[e0 + j] = l[j] > -INFINITY ? key[j] : -INFINITY;
                 }
             }
 #pragma unroll
@@ -329,14 +332,14 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, NT == 16 ? 5 : 8) route_logi
         if (a.n_groups > 1 && !lanes_of_group && !(by_logit && need_p)) {
 #pragma unroll
             for (int j = 0; j < NT; j++)
-                s_keys[lane * NT + j] = key[j];
+                s_keys[e0 + j] = key[j];
         }
         {
             int place[NT];
             places_of<NT>(key, place);
 #pragma unroll
             for (int j = 0; j < NT; j++)
-                sorted[place[j]][lane] = make_float2(key[j], __int_as_float(lane * NT + j));
+                sorted[place[j]][lane] = make_float2(key[j], __int_as_float(e0 + j));
         }
         __syncwarp();
 
@@ -347,7 +350,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, NT == 16 ? 5 : 8) route_logi
             }
             int g = lane;  // the group whose score this lane has
             if (lanes_of_group) {
-                g = lane / span;
+                g = lane >> a.lane_shift;
                 for (int o = 1; o < span; o <<= 1) {
                     const float ob = __shfl_xor_sync(0xffffffffu, group_best, o);
                     const float on = __shfl_xor_sync(0xffffffffu, group_next, o);
@@ -448,9 +451,8 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, NT == 16 ? 5 : 8) route_logi
                 double full = 0.0;
                 if (!a.sigmoid) {
 #pragma unroll 1
-                    for (int j = 0; j < NT; j++) {
-                        const int i = lane * NT + j;
-                        const float v = i < a.E ? route_logit(load_as_float(a.logits, at + i, a.dtype)) : -INFINITY;
+                    for (int j = 0; j < have; j++) {
+                        const float v = route_logit(load_as_float(a.logits, at + e0 + j, a.dtype));
                         if (v > -INFINITY)
                             full += exp((double)v - (double)lmax);
                     }

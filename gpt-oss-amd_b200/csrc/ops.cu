@@ -191,12 +191,16 @@ moe_b200_status moe_b200_route_logits(const moe_b200_route_logits_args* args, mo
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (n_tokens == 0)
         return launched("moe_b200_route_logits: counts", cudaMemsetAsync(expert_counts, 0, sizeof(int) * (size_t)E, st));
-    LogitsArgs a{logits, stride, dtype, n_tokens, E, K, score == MOE_B200_SCORE_SIGMOID, bias, n_groups, topk_groups,
-                 group_top, renormalize != 0, scale, topk_i, topk_w, expert_counts, 0};
-    const int want = (n_tokens + ROUTE_WARPS - 1) / ROUTE_WARPS, most = 8 * sms;
     const int nt = E <= 32 ? 1 : E <= 64 ? 2 : E <= 128 ? 4 : E <= 256 ? 8 : 16;
+    int lane_shift = 5;
+    while (n_groups << lane_shift > 32)
+        lane_shift--;
+    const bool by_lanes = nt << lane_shift >= E / n_groups;
+    LogitsArgs a{logits, stride, dtype, n_tokens, E, K, score == MOE_B200_SCORE_SIGMOID, bias, n_groups, topk_groups,
+                 group_top, by_lanes ? lane_shift : 5, by_lanes ? n_groups : 1, by_lanes ? E / n_groups : E, renormalize != 0, scale, topk_i, topk_w, expert_counts, 0};
+    const int want = (n_tokens + ROUTE_WARPS - 1) / ROUTE_WARPS, most = 8 * sms;
     const int piece = nt * size_of(dtype) < 16 ? nt * size_of(dtype) : 16;
-    const bool vec = E % nt == 0 && rows_aligned(logits, n_tokens, stride, size_of(dtype), piece);
+    const bool vec = a.lane_size % nt == 0 && rows_aligned(logits, n_tokens, stride, size_of(dtype), piece);
     auto kernel = nt == 1 ? (vec ? route_logits_kernel<1, true> : route_logits_kernel<1, false>)
                   : nt == 2 ? (vec ? route_logits_kernel<2, true> : route_logits_kernel<2, false>)
                   : nt == 4 ? (vec ? route_logits_kernel<4, true> : route_logits_kernel<4, false>)

@@ -194,6 +194,25 @@ def test_route_logits(T, E, k, dtype, case):
     _check_route(logits, k, r, **kw)
 
 
+@pytest.mark.parametrize("E,G", [(240, 4), (304, 4), (288, 8), (60, 6), (120, 3), (510, 3), (490, 7), (96, 32), (31, 31), (320, 5),
+                                 (72, 8), (40, 2), (511, 7), (62, 2), (130, 2), (258, 2)])
+@pytest.mark.parametrize("kw", [dict(bias=True, group_top=2), dict(score="sigmoid", bias=True, group_top=1), dict(group_top=2),
+                                dict(score="sigmoid", group_top=1)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_route_logits_groups_of_any_size(E, G, kw, dtype):
+    """Groups that fill their lanes, that leave some empty, and that share lanes."""
+    g = _gen(E + G)
+    kw = dict(kw, n_groups=G, topk_groups=(G + 1) // 2, group_top=min(kw["group_top"], E // G))
+    k = min(8, E // G * kw["topk_groups"])
+    logits = (1.5 * _randn(g, 33, E)).to(dtype)
+    logits[3, : E // 2] = -math.inf
+    logits[4, ::3] = logits[4, 0]
+    if kw.get("bias"):
+        kw["bias"] = 0.1 * _randn(g, E)
+    r = pkg.route_logits(logits, k, counts=True, **kw)
+    _check_route(logits, k, r, **kw)
+
+
 @pytest.mark.parametrize("kw", [dict(), dict(score="sigmoid"), dict(renormalize=False), dict(score="sigmoid", bias=True),
                                 dict(score="sigmoid", bias=True, n_groups=5, topk_groups=2, group_top=2),
                                 dict(n_groups=5, topk_groups=2, group_top=2), dict(n_groups=5, topk_groups=2, group_top=1)])
