@@ -11,13 +11,12 @@
 // 64-bit keys, a few tokens in a thousand for fp32 logits; where it hung on the groups, or on more
 // than 32 experts, it does the token again in 64 bits (route_exact).
 //
-// A warp owns a token; a lane holds NT neighbouring experts, lanes and experts in the same order, so the
-// lowest lane of a tie has the lowest index.  Where NT allows it every group has 2^n lanes of its own, the last
-// of them empty if need be, and is scored and dropped by lanes (240 experts in 4 groups, 4096 tokens: 11.6 us
-// without, 7.8 with).  Each lane puts its keys in order once, by counting for each
-// the keys in front of it; then a round per selected expert takes the largest of the 32 heads (one
-// warp reduction) and the winner moves on to its next key.  The logits are read once, 16 bytes a
-// lane where they are aligned.
+// A warp owns a token; a lane holds NT neighbouring experts, lanes and experts in the same order, so the lowest
+// lane of a tie has the lowest index.  Where NT allows it every group has 2^n lanes of its own, the last of them
+// empty if need be, and is scored and dropped by lanes (240 experts in 4 groups, 4096 tokens: 11.6 us without,
+// 7.8 with).  Each lane puts its keys in order once, by counting for each the keys in front of it; then a round
+// per selected expert takes the largest of the 32 heads (one warp reduction) and the winner moves on to its next
+// key.  The logits are read once, 16 bytes a lane where they are aligned.
 //
 // Bound by instruction issue for many tokens: 725 instructions per token of 256 experts with bias, top 8,
 // 16384 tokens in 16.0 us with fp32 logits (16.8 MB, 2.5 us at the HBM rate).  The order by a sorting
@@ -25,8 +24,6 @@
 // the latency of load, order and rounds: one token 2.2 us, launch included.
 #pragma once
 #include <float.h>
-
-#include <type_traits>
 
 #include "common.cuh"
 #include "op_types.cuh"
@@ -166,30 +163,36 @@ __device__ __forceinline__ float route_sigmoid(float x) {
 // 5.0; 2048 5.6, 5.4, 5.5; 4736 9.2, 7.8, 7.6; 16384 20.7, 17.0, 17.6.  Registers for eight blocks of 4 per SM: 16.0.
 constexpr int ROUTE_WARPS = 4;
 
-// Places of a lane's keys in falling order, ties by index, four bits each: a key's place is the number of keys
+// Places of N of a lane's keys in falling order, ties by index, four bits each: a key's place is the number of keys
 // in front of it, and a comparison of two moves one of them a place back.
-template <int NT>
-__device__ __forceinline__ void places_of(const float (&key)[NT], int (&place)[NT]) {
-    typedef typename std::conditional<NT == 16, unsigned long long, unsigned>::type Packed;
-    Packed packed = 0;
+template <int N>
+__device__ __forceinline__ void places_of(const float* key, int* place) {
+    unsigned packed = 0;
 #pragma unroll
-    for (int i = 0; i < NT; i++)
-        packed |= (Packed)(NT - 1 - i) << (4 * i);
+    for (int i = 0; i < N; i++)
+        packed |= (unsigned)(N - 1 - i) << (4 * i);
 #pragma unroll
-    for (int j = 1; j < NT; j++)
+    for (int j = 1; j < N; j++)
 #pragma unroll
         for (int i = 0; i < j; i++)
             if (key[i] >= key[j])
-                packed += ((Packed)1 << (4 * j)) - ((Packed)1 << (4 * i));
+                packed += (1u << (4 * j)) - (1u << (4 * i));
 #pragma unroll
-    for (int i = 0; i < NT; i++)
+    for (int i = 0; i < N; i++)
         place[i] = (int)(packed >> (4 * i)) & 15;
 }
+
+// A lane's keys lie in lists of up to 8 in order: 16 keys in one list are 120 comparisons, in two 56 and a comparison
+// of their heads per round (4096 tokens, 304 experts, top 10: 11.1 us, 9.4).
+template <int NT>
+struct RouteLists {
+    static constexpr int N = NT < 8 ? NT : 8, LISTS = NT / N, ROWS = LISTS * (N + 1);  // each with -inf at its end
+};
 
 // Dynamic shared memory of a warp: its keys in order, and route_exact's.
 template <int NT>
 __host__ __device__ constexpr size_t route_smem_bytes() {
-    return (NT + 1) * 32 * sizeof(float2) + NT * 32 * sizeof(double);
+    return RouteLists<NT>::ROWS * 32 * sizeof(float2) + NT * 32 * sizeof(double);
 }
 
 // VEC: a lane's logits are one aligned piece of memory.
@@ -199,7 +202,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, NT == 16 ? 5 : 8) route_logi
     extern __shared__ double s_dyn[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float2(*sorted)[32] = reinterpret_cast<float2(*)[32]>(s_dyn + warp * (route_smem_bytes<NT>() / 8));  // place, lane
-    double* s_keys = reinterpret_cast<double*>(sorted + NT + 1);
+    double* s_keys = reinterpret_cast<double*>(sorted + RouteLists<NT>::ROWS);
     pdl_wait();
     if (a.early)
         pdl_trigger();
@@ -220,7 +223,10 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, NT == 16 ? 5 : 8) route_logi
         const float b = a.bias && j < have ? a.bias[e0 + j] : 0.f;
         bias[j] = b > -INFINITY ? fminf(b, FLT_MAX) : -INFINITY;
     }
-    sorted[NT][lane] = make_float2(-INFINITY, 0.f);
+    constexpr int LN = RouteLists<NT>::N, LISTS = RouteLists<NT>::LISTS;
+#pragma unroll
+    for (int i = 0; i < LISTS; i++)
+        sorted[i * (LN + 1) + LN][lane] = make_float2(-INFINITY, 0.f);
     int* sel = s_sel[warp];
     for (int t = blockIdx.x * ROUTE_WARPS + warp; t < a.T; t += gridDim.x * ROUTE_WARPS) {
         float l[NT];
@@ -336,10 +342,12 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, NT == 16 ? 5 : 8) route_logi
         }
         {
             int place[NT];
-            places_of<NT>(key, place);
+#pragma unroll
+            for (int i = 0; i < LISTS; i++)
+                places_of<LN>(key + i * LN, place + i * LN);
 #pragma unroll
             for (int j = 0; j < NT; j++)
-                sorted[place[j]][lane] = make_float2(key[j], __int_as_float(e0 + j));
+                sorted[j / LN * (LN + 1) + place[j]][lane] = make_float2(key[j], __int_as_float(e0 + j));
         }
         __syncwarp();
 
@@ -347,6 +355,11 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, NT == 16 ? 5 : 8) route_logi
             if (!by_logit || !need_p) {
                 group_best = sorted[0][lane].x;
                 group_next = sorted[1][lane].x;  // NT = 1: -inf
+                if (LISTS > 1) {
+                    const float ob = sorted[LN + 1][lane].x, on = sorted[LN + 2][lane].x;
+                    group_next = fmaxf(fminf(group_best, ob), fmaxf(group_next, on));
+                    group_best = fmaxf(group_best, ob);
+                }
             }
             int g = lane;  // the group whose score this lane has
             if (lanes_of_group) {
@@ -386,19 +399,25 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, NT == 16 ? 5 : 8) route_logi
             }
             if (lanes_of_group) {
                 if (!in)
-                    sorted[0][lane].x = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < LISTS; i++)
+                        sorted[i * (LN + 1)][lane].x = -INFINITY;
             } else {
                 const unsigned kept = __ballot_sync(0xffffffffu, in);
-                int n = 0;
 #pragma unroll 1
-                for (int j = 0; j < NT; j++) {  // those that stay move up
-                    const float2 v = sorted[j][lane];
-                    const int e = __float_as_int(v.y);
-                    if (v.x > -INFINITY && e < a.E && ((kept >> (e / gs)) & 1u))
-                        sorted[n++][lane] = v;
+                for (int i = 0; i < LISTS; i++) {
+                    float2(*list)[32] = sorted + i * (LN + 1);
+                    int n = 0;
+#pragma unroll 1
+                    for (int j = 0; j < LN; j++) {  // those that stay move up
+                        const float2 v = list[j][lane];
+                        const int e = __float_as_int(v.y);
+                        if (v.x > -INFINITY && e < a.E && ((kept >> (e / gs)) & 1u))
+                            list[n++][lane] = v;
+                    }
+                    for (int j = n; j < LN; j++)
+                        list[j][lane].x = -INFINITY;
                 }
-                for (int j = n; j < NT; j++)
-                    sorted[j][lane].x = -INFINITY;
             }
         }
 
@@ -407,16 +426,34 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, NT == 16 ? 5 : 8) route_logi
         float2 head = sorted[0][lane];
         float mine_key = -INFINITY;
         const float2* next = &sorted[1][lane];
+        float2 other = make_float2(-INFINITY, 0.f);  // the second list's head; `head` is the larger, the first list's in a tie
+        const float2* other_next = nullptr;
+        bool second = false;
+        auto larger = [&]() {
+            if (second ? other.x >= head.x : other.x > head.x) {
+                const float2 h = head;
+                const float2* n = next;
+                head = other, next = other_next, other = h, other_next = n;
+                second = !second;
+            }
+        };
+        if (LISTS > 1) {
+            other = sorted[LN + 1][lane];
+            other_next = &sorted[LN + 2][lane];
+            larger();
+        }
         const unsigned lower = (1u << lane) - 1u;
         auto round = [&](int k) {
             const float top = warp_best(head.x);
             const unsigned has = __ballot_sync(0xffffffffu, head.x == top);
             if (lane == k)
                 mine_key = top;
-            if (head.x == top && top > -INFINITY && !(has & lower)) {  // at most NT times: place NT holds -inf
+            if (head.x == top && top > -INFINITY && !(has & lower)) {  // a list ends with -inf
                 sel[k] = __float_as_int(head.y);
                 head = *next;
                 next += 32;
+                if (LISTS > 1)
+                    larger();
             }
             return top;
         };
