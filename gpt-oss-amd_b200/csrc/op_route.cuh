@@ -18,7 +18,7 @@
 // per selected expert takes the largest of the 32 heads (one warp reduction) and the winner moves on to its next
 // key.  The logits are read once, 16 bytes a lane where they are aligned.
 //
-// Bound by instruction issue for many tokens: 725 instructions per token of 256 experts with bias, top 8,
+// Bound by instruction issue for many tokens: 749 instructions per token of 256 experts with bias, top 8,
 // 16384 tokens in 16.0 us with fp32 logits (16.8 MB, 2.5 us at the HBM rate).  The order by a sorting
 // network of 19 exchanges took 19.1, a search over all keys per round 44.  Few tokens are bound by
 // the latency of load, order and rounds: one token 2.2 us, launch included.
