@@ -301,8 +301,11 @@ __global__ void __launch_bounds__(MV_BLOCK, 2) w4_matvec_kernel(const __grid_con
             const uint8_t* s = static_cast<const uint8_t*>(a.scales) + row0 * SG * SB;
             const int scales = l_c0 == 0 ? rows * SG * SB : 0, bulk = a.scale_bulk ? scales & ~15 : 0;
             const int to = scales_at + l_slot * a.scale_slot;
-            for (int i = bulk + lane; i < scales; i += 32)  // what no bulk copy may take
-                dyn[to + i] = s[i];
+            if (bulk < scales) {  // what no bulk copy may take; a later tile's may be written over it, after these stores
+                for (int i = bulk + lane; i < scales; i += 32)
+                    dyn[to + i] = s[i];
+                fence_proxy_async_smem();
+            }
             __syncwarp();
             if (lane == 0)
                 mbar_expect_tx(full, rows * pieces * 16 + bulk);
