@@ -379,7 +379,11 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, NT == 16 ? 5 : 8) route_logi
                         group_best = fmaxf(group_best, v);
                     }
             }
-            const float score = g < a.n_groups ? (a.group_top > 1 && group_next > -INFINITY ? group_best + group_next : group_best) : -INFINITY;
+            // Keys are finite, but the sum of two may not be in fp32: such a group counts as the lowest or the largest, it is
+            // not out, and the order of several of them is for 64 bits.
+            const bool live = g < a.n_groups && group_best > -INFINITY;
+            const float sum2 = a.group_top > 1 && group_next > -INFINITY ? group_best + group_next : group_best;
+            const float score = live ? fmaxf(sum2, -FLT_MAX) : -INFINITY;
             // a group's place: the groups in front of it
             int place = 0;
             const int step = lanes_of_group ? span : 1;
@@ -387,9 +391,9 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, NT == 16 ? 5 : 8) route_logi
                 const float o = __shfl_sync(0xffffffffu, score, i * step);
                 place += o > score || (o == score && i < g);
             }
-            const bool in = score > -INFINITY && place < a.topk_groups;
+            const bool in = live && place < a.topk_groups;
             if (!(by_logit && a.group_top == 1) && a.topk_groups < a.n_groups) {
-                const float low = -warp_best(in && g < a.n_groups ? -score : -INFINITY);
+                const float low = -warp_best(in ? -score : -INFINITY);
                 const float high = warp_best(!in && g < a.n_groups ? score : -INFINITY);
                 // a score is off by its two keys' errors and a rounding; the keys may be far larger than their sum
                 const float big = warp_best(fmaxf(group_best > -INFINITY ? fabsf(group_best) : 0.f,
