@@ -15,9 +15,12 @@
 // the four accumulators of a lane are multiplied by x scale and weight scale into fp32 sums.
 //
 // x is rounded to nothing: bf16 becomes fp16 after the group of 32 was multiplied by the power of two
-// that brings its largest value to [2^14, 2^15), which the x scale of the group takes back (exact but for
-// values 2^-38 below the group's largest); e4m3 is a subset of fp16.  Code values are exact in
-// fp16, so each product is exact and the sums are fp32.
+// that brings its largest value to [2^14, 2^15), which the x scale of the group takes back; e4m3 is a subset of
+// fp16.  Code values are exact in fp16, so each product is exact and the sums are fp32.
+// What does not fit is "far" and stays out of the MMA: in bf16, values more than 2^31 below their group's largest
+// (the 8 bits of the others end at 2^-24 or above, where fp16's do), and whole groups whose x scale is not within
+// 2^-100..2^103: the products of a group are multiples of 2^-25 and sum to less than 2^24, so with a scale inside
+// they stay exact, and finite, before the weight scale joins.  The warps add what is far at the end of a tile, in 64 bits.
 //
 // The stream.  A ninth warp feeds a ring of up to four stages in shared memory with bulk copies: one
 // copy for the codes of a tile of 16 rows, which lie together, and one for its scales; the eight others take the
@@ -36,6 +39,8 @@
 #include "common.cuh"
 #include "op_types.cuh"
 #include "tc5_ptx.cuh"
+
+#include <cuda_fp8.h>
 
 namespace moe {
 namespace op {
@@ -163,25 +168,69 @@ __device__ __forceinline__ uint32_t mv_load_scales(const uint8_t* row, int sg, i
     return r;
 }
 
-// One row of x in fp16 and the scale of each of its groups, by all threads of the block.
+// Keeps what is computed from `v` where it stands: code that runs seldom would else have its constants computed in
+// front of the loops around it, and kept in registers through them.
+__device__ __forceinline__ void mv_opaque(int& v) { asm volatile("" : "+r"(v)); }
+
+// The x scale of a group, for rows that have some.
+__device__ __forceinline__ float mv_x_scale(const MatvecArgs& a, long long xr, int grp) {
+    const long long at = xr * a.n_xs + (a.xs_shift == 31 ? 0 : grp >> a.xs_shift);
+    return a.xs_mx ? e8m0_to_float(static_cast<const uint8_t*>(a.x_scales)[at]) : static_cast<const float*>(a.x_scales)[at];
+}
+
+// bf16: exponent field of a group's largest value (14 at least) from its magnitude bits, and what is far.
+__device__ __forceinline__ uint32_t mv_top_exponent(uint32_t top) { return max(top >> 23, 14u); }
+__device__ __forceinline__ bool mv_far_group(uint32_t top) {  // the x scale 2^(ex - 141) is out of its range
+    return top != 0 && (mv_top_exponent(top) < 41u || mv_top_exponent(top) > 244u);
+}
+__device__ __forceinline__ bool mv_far_value(uint32_t bits, uint32_t top) {
+    return (bits & 0x7FFFFFFFu) != 0 && ((bits >> 23) & 255u) + 31u < mv_top_exponent(top);
+}
+__device__ __forceinline__ bool mv_far_scale(float sc) { return !(sc == 0.f || (fabsf(sc) >= 0x1p-100f && fabsf(sc) <= 0x1p103f)); }
+
+// Largest magnitude of a group, eight values in each lane of a quad, as bits; `far`: something in it is far.
+__device__ __forceinline__ uint32_t mv_top(const uint32_t (&h)[4], int tid, bool& far) {
+    uint32_t most = 0, least = 0;  // the smallest but zero, less one, as its complement: both are maxima, of 16-bit lanes
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const uint32_t v = h[e] & 0x7FFF7FFFu;
+        most = __vmaxu2(most, v);
+        least = __vmaxu2(least, ~__vsub2(v, 0x00010001u));
+    }
+    most = __vmaxu2(__byte_perm(most, least, 0x5410), __byte_perm(most, least, 0x7632));
+    const unsigned quad = 0xFu << (tid & 28);
+    most = __vmaxu2(most, __shfl_xor_sync(quad, most, 1));
+    most = __vmaxu2(most, __shfl_xor_sync(quad, most, 2));
+    const uint32_t top = most << 16;
+    far = mv_far_group(top) || mv_far_value((~most & 0xFFFF0000u) + 0x10000u, top);
+    return top;
+}
+
+// One row of x in fp16 and the scale of each of its groups, by all threads of the block.  Returns whether this thread
+// saw something far.
 template <bool INT4>
-__device__ __forceinline__ void mv_load_x(const MatvecArgs& a, long long xr, int steps, int G, uint4* xs, float* xsc) {
-    for (int k8 = threadIdx.x; k8 < steps * 16; k8 += MV_THREADS) {  // eight columns; four lanes make a group
+__device__ __forceinline__ bool mv_load_x(const MatvecArgs& a, long long xr, int steps, int G, uint4* xs, float* xsc) {
+    bool any = false;
+    int tid = threadIdx.x;
+    mv_opaque(tid);
+    for (int k8 = tid; k8 < steps * 16; k8 += MV_THREADS) {  // eight columns; four lanes make a group
         const int grp = k8 >> 2;
         float sc = 0.f;
         uint32_t h[4] = {0, 0, 0, 0};
+        bool is_far = false;
         if (grp < G) {
-            sc = 1.f;
-            if (a.x_scales) {
-                const long long at = xr * a.n_xs + (a.xs_shift == 31 ? 0 : grp >> a.xs_shift);
-                sc = a.xs_mx ? e8m0_to_float(static_cast<const uint8_t*>(a.x_scales)[at]) : static_cast<const float*>(a.x_scales)[at];
-            }
+            sc = a.x_scales ? mv_x_scale(a, xr, grp) : 1.f;
             if (a.x_dtype == MOE_B200_DTYPE_E4M3) {
                 const uint2 q = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.x) + xr * a.x_stride + k8 * 8);
                 const uint32_t w[4] = {q.x & 0xFFFFu, q.x >> 16, q.y & 0xFFFFu, q.y >> 16};
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h[e]) : "h"((uint16_t)w[e]));
+                is_far = mv_far_scale(sc);
+                if (is_far) {
+                    h[0] = h[1] = h[2] = h[3] = 0;
+                    sc = 0.f;
+                }
             } else {
                 const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + xr * a.x_stride + k8 * 8);
                 h[0] = q.x;
@@ -191,16 +240,16 @@ __device__ __forceinline__ void mv_load_x(const MatvecArgs& a, long long xr, int
             }
         }
         if (a.x_dtype == MOE_B200_DTYPE_BF16) {
-            uint32_t m = 0;  // largest magnitude of the group, as bits
+            const uint32_t m = mv_top(h, tid, is_far);
+            const bool whole = mv_far_group(m);
+            if (is_far)
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                m = max(m, max((h[e] << 16) & 0x7FFFFFFFu, h[e] & 0x7FFF0000u));
-            const unsigned quad = 0xFu << (threadIdx.x & 28);
-            m = max(m, __shfl_xor_sync(quad, m, 1));
-            m = max(m, __shfl_xor_sync(quad, m, 2));
-            const uint32_t ex = max(m >> 23, 14u);
+                for (int e = 0; e < 4; e++)
+                    h[e] &= (whole || mv_far_value(h[e] << 16, m) ? 0u : 0x0000FFFFu) |
+                            (whole || mv_far_value(h[e] & 0xFFFF0000u, m) ? 0u : 0xFFFF0000u);
+            const uint32_t ex = mv_top_exponent(m);
             const float up = __uint_as_float((268u - ex) << 23);  // 2^(141 - ex)
-            sc = grp < G ? __uint_as_float(max((ex - 14u) << 23, 0x00400000u)) : 0.f;
+            sc = grp < G && !whole ? __uint_as_float(max((ex - 14u) << 23, 0x00400000u)) : 0.f;
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 h[e] = floats_to_half2(__uint_as_float(h[e] << 16) * up, __uint_as_float(h[e] & 0xFFFF0000u) * up, MOE_B200_DTYPE_F16);
@@ -216,224 +265,126 @@ __device__ __forceinline__ void mv_load_x(const MatvecArgs& a, long long xr, int
         xs[k8] = make_uint4(h[0], h[1], h[2], h[3]);
         if ((k8 & 3) == 0)
             xsc[grp] = sc;
+        any |= is_far;
     }
+    return any;
 }
 
-// P pairs of x rows (columns of the MMA) per pass over the weights.
-template <bool INT4, bool PAIRED, int P>
-__global__ void __launch_bounds__(MV_BLOCK, 2) w4_matvec_kernel(const __grid_constant__ MatvecArgs a) {
-    using namespace moe::tc5;
-    constexpr int RP = 2 * P;
-    constexpr int SB = INT4 ? 2 : 1;  // bytes of a scale
-    extern __shared__ __align__(128) uint8_t dyn[];
-    __shared__ __align__(8) uint64_t s_full[MV_MAX_DEPTH], s_done[MV_MAX_DEPTH];
-    __shared__ float2 s_red[MV_MAX_DEPTH][MV_WARPS][P][16];
-    __shared__ int s_ids[MV_MAX_ROWS];
-    __shared__ int s_lead[MV_MAX_ROWS];
-    __shared__ int s_rank[MV_MAX_ROWS];
-    __shared__ int s_rows[RP], s_store_rows[RP];
-    __shared__ int s_abort;
+// Groups of this warp's steps w, w + 8, ... of a row of x in which something is far: bit 4 i + j is group j of its i-th step.
+__device__ __forceinline__ unsigned long long mv_far_groups(const MatvecArgs& a, long long xr) {
+    static_assert(MOE_B200_W4_MATVEC_MAX_IN <= 16 * MV_WARPS * 128, "16 steps of 4 groups in 64 bits");
+    const int lane = threadIdx.x & 31;
+    unsigned long long all = 0;
+#pragma unroll 1
+    for (int b = threadIdx.x >> 5, at = 0; b < mv_steps(a.K); b += 2 * MV_WARPS, at += 8) {  // two steps: a group per quad
+        const int grp = (b + (lane >> 4) * MV_WARPS) * 4 + (lane >> 2 & 3);
+        uint32_t h[4] = {0, 0, 0, 0};
+        bool far = false;
+        if (grp < a.K >> 5) {
+            if (a.x_dtype == MOE_B200_DTYPE_BF16) {
+                const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + xr * a.x_stride + grp * 32 + (lane & 3) * 8);
+                h[0] = v.x, h[1] = v.y, h[2] = v.z, h[3] = v.w;
+            } else {
+                far = mv_far_scale(mv_x_scale(a, xr, grp));
+            }
+        }
+        bool far16;
+        mv_top(h, lane, far16);
+        const unsigned votes = __ballot_sync(0xffffffffu, far || far16);
+#pragma unroll
+        for (int q = 0; q < 8; q++)
+            all |= (unsigned long long)(votes >> (4 * q) & 1) << (at + q);
+    }
+    return all;
+}
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+// What is far in a row of x, in those groups, times rows n and n + 8 of a matrix; the four lanes of a quad have the
+// same n and share the 32 columns of a group.  From global memory.
+template <bool INT4>
+__device__ __forceinline__ float2 mv_far(const MatvecArgs& a, int mat, int n, long long xr, unsigned long long groups) {
+    const int lane = threadIdx.x & 31, t = lane & 3, G = a.K >> 5, SG = G >> a.group_shift;
+    const bool bf16 = a.x_dtype == MOE_B200_DTYPE_BF16;
+    auto weight = [](uint32_t n) {
+        if (INT4)
+            return (float)((int)n - 8);
+        const uint32_t m = n & 7;
+        const float v = m < 2 ? 0.5f * m : 0.25f * ((2 + (m & 1)) << (m >> 1));
+        return n & 8 ? -v : v;
+    };
+    auto scale = [&](size_t i) {
+        return INT4 ? half_to_float(static_cast<const uint16_t*>(a.scales)[i], MOE_B200_DTYPE_BF16)
+                    : e8m0_to_float(static_cast<const uint8_t*>(a.scales)[i]);
+    };
+    double lo = 0.0, hi = 0.0;
+#pragma unroll 1
+    for (; groups; groups &= groups - 1) {
+        const int at = __ffsll(groups) - 1, grp = ((int)(threadIdx.x >> 5) + (at >> 2) * MV_WARPS) * 4 + (at & 3);
+        const long long col = xr * a.x_stride + grp * 32 + t * 8;
+        const size_t row0 = (size_t)mat * a.N + min(n, a.N - 1), row1 = (size_t)mat * a.N + min(n + 8, a.N - 1);
+        uint32_t w0 = *reinterpret_cast<const uint32_t*>(a.codes + (row0 * G + grp) * 16 + t * 4);
+        uint32_t w1 = *reinterpret_cast<const uint32_t*>(a.codes + (row1 * G + grp) * 16 + t * 4);
+        const float s0 = scale(row0 * SG + (grp >> a.group_shift)), s1 = scale(row1 * SG + (grp >> a.group_shift));
+        uint32_t top = 0;
+        bool whole = true;
+        if (bf16) {
+            const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + col);
+            const uint32_t h[4] = {v.x, v.y, v.z, v.w};
+            top = mv_top(h, lane, whole);
+            whole = mv_far_group(top);
+        }
+        double d0 = 0.0, d1 = 0.0;
+#pragma unroll 1
+        for (int i = 0; i < 8; i++) {
+            float x;
+            if (bf16) {
+                const uint32_t bits = (uint32_t)static_cast<const uint16_t*>(a.x)[col + i] << 16;
+                x = whole || mv_far_value(bits, top) ? __uint_as_float(bits) : 0.f;
+            } else {
+                __nv_fp8_e4m3 v;
+                v.__x = static_cast<const uint8_t*>(a.x)[col + i];
+                x = (float)v;
+            }
+            d0 += (double)weight(w0 & 15) * (double)x;
+            d1 += (double)weight(w1 & 15) * (double)x;
+            w0 >>= 4, w1 >>= 4;
+        }
+        const double sx = bf16 ? 1.0 : (double)mv_x_scale(a, xr, grp);
+        d0 *= sx * (double)s0, d1 *= sx * (double)s1;
+        d0 += __shfl_xor_sync(0xffffffffu, d0, 1), d1 += __shfl_xor_sync(0xffffffffu, d1, 1);
+        lo += d0 + __shfl_xor_sync(0xffffffffu, d0, 2), hi += d1 + __shfl_xor_sync(0xffffffffu, d1, 2);
+    }
+    return make_float2((float)lo, (float)hi);
+}
+
+// Shared memory of the kernel beside the dynamic part.
+template <int P>
+struct MvShared {
+    alignas(8) uint64_t full[MV_MAX_DEPTH], done[MV_MAX_DEPTH];
+    float2 red[MV_MAX_DEPTH][MV_WARPS][P][16];
+    int ids[MV_MAX_ROWS];
+    int lead[MV_MAX_ROWS];
+    int rank[MV_MAX_ROWS];
+    int rows[2 * P], store_rows[2 * P];
+    int abort;
+};
+
+// Where the warps that compute are: the tiles of a pass, and the ring.
+struct MvRun {
+    int li, cnt, tile, tile_end, stage, slot;
+    uint32_t parity;
+};
+
+// The sums of the tiles of a pass.  FAR: something of its x is far.  Two instances: one with a test at the end of a tile
+// took 66 us for the vocabulary (one row, mxfp4), this takes 62.5; with one far value in x 142, with one in each of its
+// 90 groups 1200.
+template <bool INT4, bool PAIRED, int P, bool FAR>
+__device__ __forceinline__ void mv_tiles(const MatvecArgs& a, MvShared<P>& sh, uint8_t* dyn, MvRun& r) {
+    using namespace moe::tc5;
+    constexpr int RP = 2 * P, SB = INT4 ? 2 : 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int steps = mv_steps(a.K), G = a.K >> 5, SG = G >> a.group_shift, D = a.depth;
-    // dynamic shared memory: zeros, the ring of codes, that of scales, x [min(RP, R)][steps * 128] fp16, its scales
     const int stage_bytes = MV_TILE * a.pitch, scales_at = 128 + D * stage_bytes;
     const int xs_at = scales_at + a.scale_slots * a.scale_slot, xsc_at = xs_at + min(RP, a.R) * steps * 256;
-    if (tid < 4)
-        reinterpret_cast<uint4*>(dyn)[tid] = make_uint4(0, 0, 0, 0);
-    if (tid == 0) {
-        for (int i = 0; i < D; i++) {
-            mbar_init(smem_u32(&s_full[i]), 1);
-            mbar_init(smem_u32(&s_done[i]), MV_WARPS);
-        }
-        s_abort = 0;
-        fence_barrier_init();
-    }
-
-    pdl_wait();
-    pdl_trigger();
-
-    // the list of leaders: rows that open a pass over their matrix
-    int n_lead;
-    if (a.ids) {
-        int id = -1, rank = 0;
-        if (tid < a.R) {
-            id = a.ids[tid];
-            if (id < 0 || id >= a.n_mats)
-                id = -1;
-            s_ids[tid] = id;
-        }
-        __syncthreads();
-        if (id >= 0)
-            for (int j = 0; j < tid; j++)
-                rank += s_ids[j] == id;
-        if (tid < a.R)
-            s_rank[tid] = id >= 0 ? rank : -1;
-        __syncthreads();
-        n_lead = 0;
-        for (int m0 = 0; m0 < a.R; m0 += 32) {  // every warp finds the same
-            const int m = m0 + lane;
-            const bool lead = m < a.R && s_rank[m] >= 0 && s_rank[m] % RP == 0;
-            const unsigned votes = __ballot_sync(0xffffffffu, lead);
-            if (lead)
-                s_lead[n_lead + __popc(votes & ((1u << lane) - 1u))] = m;
-            n_lead += __popc(votes);
-        }
-    } else {
-        n_lead = (a.R + RP - 1) / RP;
-    }
-    __syncthreads();
-    const long long total = (long long)n_lead * a.n_tiles;  // fits an int (checked by the host)
-    const int i0 = (int)(total * blockIdx.x / gridDim.x), i1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
-    const int li0 = i0 / a.n_tiles, tile0 = i0 - li0 * a.n_tiles;
-
-    if (warp == MV_WARPS) {
-        // ---- feeds the ring, and stores the tiles that the others have summed ----
-        // A stage is free, and its tile's sums are complete, when the eight warps have arrived on `done`.
-        int l_left = i1 - i0, l_li = li0, l_tile = tile0, l_c0 = 0, l_stage = 0, l_slot = 0;
-        auto load = [&]() {
-            if (l_left <= 0)
-                return;
-            const size_t row0 = (size_t)(a.ids ? s_ids[s_lead[l_li]] : 0) * a.N + l_tile * MV_TILE;
-            const int rows = min(MV_TILE, a.N - l_tile * MV_TILE);
-            const int pieces = min(a.chunk_steps * 4, G - l_c0 * 4);  // of 16 bytes
-            const uint32_t full = smem_u32(&s_full[l_stage]);
-            const uint8_t* s = static_cast<const uint8_t*>(a.scales) + row0 * SG * SB;
-            const int scales = l_c0 == 0 ? rows * SG * SB : 0, bulk = a.scale_bulk ? scales & ~15 : 0;
-            const int to = scales_at + l_slot * a.scale_slot;
-            if (bulk < scales) {  // what no bulk copy may take; a later tile's may be written over it, after these stores
-                for (int i = bulk + lane; i < scales; i += 32)
-                    dyn[to + i] = s[i];
-                fence_proxy_async_smem();
-            }
-            __syncwarp();
-            if (lane == 0)
-                mbar_expect_tx(full, rows * pieces * 16 + bulk);
-            __syncwarp();
-            if (a.chunk_steps == steps) {  // whole rows, as they lie
-                if (lane == 0)
-                    bulk_load(smem_u32(dyn) + 128 + l_stage * stage_bytes, a.codes + row0 * G * 16, rows * G * 16, full);
-            } else if (lane < rows)
-                bulk_load(smem_u32(dyn) + 128 + l_stage * stage_bytes + lane * a.pitch,
-                          a.codes + ((row0 + lane) * G + l_c0 * 4) * 16, pieces * 16, full);
-            if (lane == 31 && bulk)
-                bulk_load(smem_u32(dyn) + to, s, bulk, full);
-            l_stage = l_stage + 1 == D ? 0 : l_stage + 1;
-            l_c0 += a.chunk_steps;
-            if (l_c0 >= steps) {
-                l_c0 = 0;
-                l_left--;
-                l_slot = l_slot + 1 == a.scale_slots ? 0 : l_slot + 1;
-                if (++l_tile == a.n_tiles) {
-                    l_tile = 0;
-                    l_li++;
-                }
-            }
-        };
-        for (int i = 0; i < D; i++)
-            load();
-        int li = li0, tile = tile0, stage = 0, cur_lead = -1, cnt = 0, mat = 0;
-        uint32_t parity = 0;
-        bool ok = true;
-        for (int item = i0; item < i1; item++) {
-            if (li != cur_lead) {  // the rows of this pass
-                cur_lead = li;
-                __syncwarp();
-                if (a.ids) {
-                    const int first = s_rank[s_lead[li]];
-                    mat = s_ids[s_lead[li]];
-                    cnt = 0;
-                    for (int m0 = 0; m0 < a.R; m0 += 32) {
-                        const int m = m0 + lane;
-                        const bool in = m < a.R && s_ids[m] == mat && s_rank[m] >= first && s_rank[m] < first + RP;
-                        if (in)
-                            s_store_rows[s_rank[m] - first] = m;
-                        cnt += __popc(__ballot_sync(0xffffffffu, in));
-                    }
-                } else {
-                    cnt = min(RP, a.R - li * RP);
-                    if (lane < cnt)
-                        s_store_rows[lane] = li * RP + lane;
-                }
-                __syncwarp();
-            }
-            float bias[2];
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                const int n = tile * MV_TILE + g + 8 * half;
-                bias[half] = a.bias && n < a.N ? a.bias[(size_t)mat * a.N + n] : 0.f;
-            }
-            float2 v[P];
-            for (int c0 = 0; c0 < steps; c0 += a.chunk_steps) {
-                ok = ok && mbar_wait(smem_u32(&s_done[stage]), parity, nullptr, 0, &s_abort) &&
-                     *(volatile int*)&s_abort == 0;
-                ok = __all_sync(0xffffffffu, ok);
-                if (c0 + a.chunk_steps >= steps) {
-                    // lane: row g of both halves, x row 2 p + t / 2 (the same in lanes t and t ^ 1); warps in order
-#pragma unroll
-                    for (int p = 0; p < P; p++) {
-                        v[p] = make_float2(0.f, 0.f);
-#pragma unroll
-                        for (int w = 0; w < MV_WARPS; w++) {
-                            const float2 r = s_red[stage][w][p][lane >> 1];
-                            v[p].x += r.x;
-                            v[p].y += r.y;
-                        }
-                    }
-                    __syncwarp();
-                }
-                if (ok)
-                    load();
-                if (++stage == D) {
-                    stage = 0;
-                    parity ^= 1;
-                }
-            }
-            const float poison = ok ? 0.f : __int_as_float(0x7FC00000);  // a wait that ran out leaves NaN
-#pragma unroll
-            for (int p = 0; p < P; p++) {
-                if (2 * p >= cnt)
-                    break;
-                const int c = 2 * p + (t >> 1);
-                const long long row = (long long)s_store_rows[min(c, cnt - 1)] * a.out_stride;
-#pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    const int n = tile * MV_TILE + g + 8 * half;
-                    const float s = (half ? v[p].y : v[p].x) + bias[half] + poison;
-                    const float up_raw = __shfl_down_sync(0xffffffffu, s, 4);  // row g + 1
-                    if ((t & 1) == 0 && c < cnt && n < a.N) {
-                        if (!a.swiglu) {
-                            store_from_float(a.out, row + n, a.out_dtype, s);
-                        } else if ((g & 1) == 0) {
-                            const float gt = s > a.limit ? a.limit : s;  // comparisons that let NaN through
-                            const float up = up_raw > a.limit ? a.limit : up_raw < -a.limit ? -a.limit : up_raw;
-                            store_from_float(a.out, row + (n >> 1), a.out_dtype, gt / (1.f + expf(-a.alpha * gt)) * (up + 1.f));
-                        }
-                    }
-                }
-            }
-            if (++tile == a.n_tiles) {
-                tile = 0;
-                li++;
-            }
-        }
-        if (!ok)  // copies that are still on their way get a bounded time to land
-            for (int i = 0; i < D; i++) {
-                drain_wait(smem_u32(&s_full[i]), 0);
-                drain_wait(smem_u32(&s_full[i]), 1);
-            }
-        // rows without a matrix
-        if (a.ids) {
-            const int n_out = a.swiglu ? a.N >> 1 : a.N;
-            for (int m = 0; m < a.R; m++)
-                if (s_ids[m] < 0)
-                    for (long long n = (long long)blockIdx.x * 32 + lane; n < n_out; n += (long long)gridDim.x * 32)
-                        store_from_float(a.out, m * a.out_stride + n, a.out_dtype, 0.f);
-        }
-        return;
-    }
-
-    // ---- computes ----
     // Lanes g of the MMA take row gr of each half: eight lanes that read shared memory together have two rows, g even
     // and g + 1, and these should lie 64 bytes apart modulo 128.
     const int gr = a.row_map == 1 ? (g & 4) | (g & 1) << 1 | (g >> 1 & 1) : a.row_map == 2 ? (g & 1) << 2 | g >> 1 : g;
@@ -447,56 +398,27 @@ __global__ void __launch_bounds__(MV_BLOCK, 2) w4_matvec_kernel(const __grid_con
     for (int k = 0; k < 4; k++)
         x1[k] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-    for (int p = 0; p < P; p++)
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-            acc[p][k] = 0.f;
-    int li = li0, tile = tile0, stage = 0, slot = 0, cur_lead = -1, cnt = 0;
-    uint32_t parity = 0;
-    for (int item = i0; item < i1; item++) {
-        if (li != cur_lead) {
-            // the rows of this pass, their x in fp16 and its scales
-            cur_lead = li;
-            asm volatile("bar.sync 1, %0;" ::"n"(MV_THREADS) : "memory");  // nobody computes with the last ones
-            if (a.ids) {
-                const int first = s_rank[s_lead[li]], mat = s_ids[s_lead[li]];
-                cnt = 0;
-                for (int m0 = 0; m0 < a.R; m0 += 32) {  // every warp counts, each stores the same
-                    const int m = m0 + lane;
-                    const bool in = m < a.R && s_ids[m] == mat && s_rank[m] >= first && s_rank[m] < first + RP;
-                    if (in)
-                        s_rows[s_rank[m] - first] = m;
-                    cnt += __popc(__ballot_sync(0xffffffffu, in));
-                }
-            } else {
-                cnt = min(RP, a.R - li * RP);
-                if (lane < cnt)
-                    s_rows[lane] = li * RP + lane;
-            }
-            __syncwarp();
-            for (int c = 0; c < cnt; c++)
-                mv_load_x<INT4>(a, s_rows[c] / a.rows_per_x, steps, G, reinterpret_cast<uint4*>(dyn + xs_at) + c * steps * 16,
-                                reinterpret_cast<float*>(dyn + xsc_at) + c * steps * 4);
-            asm volatile("bar.sync 1, %0;" ::"n"(MV_THREADS) : "memory");
-#pragma unroll
-            for (int p = 0; p < P; p++) {
-                const int c = 2 * p + (g >> 2), cs = 2 * p + (t >> 1);
-                const bool mine = quad_b && c < cnt;
-                x_at[p] = mine ? xs_at + (c * steps * 16 + t * 4) * 16 : 0;
-                x_step[p] = mine ? 256 : 0;
-                sc_at[p] = xsc_at + (min(cs, cnt - 1) * steps * 4 + 2 * (t & 1)) * 4;
-                if (P == 1 && !mine)
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        x1[k] = make_uint4(0, 0, 0, 0);
-            }
-        }
-        const int scales_row = scales_at + slot * a.scale_slot + gr * SG * SB;
+    for (int p = 0; p < P; p++) {
+        const int c = 2 * p + (g >> 2), cs = 2 * p + (t >> 1);
+        const bool mine = quad_b && c < r.cnt;
+        x_at[p] = mine ? xs_at + (c * steps * 16 + t * 4) * 16 : 0;
+        x_step[p] = mine ? 256 : 0;
+        sc_at[p] = xsc_at + (min(cs, r.cnt - 1) * steps * 4 + 2 * (t & 1)) * 4;
+        acc[p][0] = acc[p][1] = acc[p][2] = acc[p][3] = 0.f;
+    }
+    unsigned long long far[RP];
+    if constexpr (FAR)
+#pragma unroll 1
+        for (int c = 0; c < r.cnt; c++)
+            far[c] = mv_far_groups(a, sh.rows[c] / a.rows_per_x);
+#pragma unroll 1
+    for (; r.tile < r.tile_end; r.tile++) {
+        const int scales_row = scales_at + r.slot * a.scale_slot + gr * SG * SB;
         for (int c0 = 0; c0 < steps; c0 += a.chunk_steps) {
-            mbar_wait(smem_u32(&s_full[stage]), parity, nullptr, 0, &s_abort);
+            mbar_wait(smem_u32(&sh.full[r.stage]), r.parity, nullptr, 0, &sh.abort);
             // Warp w takes the steps w, w + 8, ... of a row, whatever the chunks: a row's sums have one order.
             const int c1 = min(c0 + a.chunk_steps, steps);
-            const int codes_at = 128 + stage * stage_bytes + gr * a.pitch + t * 16 - c0 * 64;
+            const int codes_at = 128 + r.stage * stage_bytes + gr * a.pitch + t * 16 - c0 * 64;
             // offsets of the warp's step, moved on by eight steps at a time
             int b = c0 + warp, sg = b * 4 + 2 * (t & 1), code_at = codes_at + b * 64;
             int x_b[P], sc_b[P];
@@ -555,23 +477,281 @@ __global__ void __launch_bounds__(MV_BLOCK, 2) w4_matvec_kernel(const __grid_con
                     float lo = acc[p][0] + acc[p][1], hi = acc[p][2] + acc[p][3];
                     lo += __shfl_xor_sync(0xffffffffu, lo, 1);
                     hi += __shfl_xor_sync(0xffffffffu, hi, 1);
+                    if constexpr (FAR)
+#pragma unroll 1
+                        for (int c = 2 * p; c < min(2 * p + 2, r.cnt); c++) {
+                            const float2 f = mv_far<INT4>(a, a.ids ? sh.ids[sh.lead[r.li]] : 0, r.tile * MV_TILE + gr, sh.rows[c] / a.rows_per_x, far[c]);
+                            if (c == 2 * p + (t >> 1)) {
+                                lo += f.x;
+                                hi += f.y;
+                            }
+                        }
                     if ((t & 1) == 0)
-                        s_red[stage][warp][p][gr * 2 + (t >> 1)] = make_float2(lo, hi);
+                        sh.red[r.stage][warp][p][gr * 2 + (t >> 1)] = make_float2(lo, hi);
                     acc[p][0] = acc[p][1] = acc[p][2] = acc[p][3] = 0.f;
                 }
             }
             __syncwarp();  // all lanes have read the stage and left their sums
             if (lane == 0)
-                mbar_arrive(smem_u32(&s_done[stage]));
-            if (++stage == D) {
-                stage = 0;
-                parity ^= 1;
+                mbar_arrive(smem_u32(&sh.done[r.stage]));
+            if (++r.stage == D) {
+                r.stage = 0;
+                r.parity ^= 1;
             }
         }
-        slot = slot + 1 == a.scale_slots ? 0 : slot + 1;
-        if (++tile == a.n_tiles) {
-            tile = 0;
-            li++;
+        r.slot = r.slot + 1 == a.scale_slots ? 0 : r.slot + 1;
+    }
+}
+
+// P pairs of x rows (columns of the MMA) per pass over the weights.
+template <bool INT4, bool PAIRED, int P>
+__global__ void __launch_bounds__(MV_BLOCK, 2) w4_matvec_kernel(const __grid_constant__ MatvecArgs a) {
+    using namespace moe::tc5;
+    constexpr int RP = 2 * P;
+    constexpr int SB = INT4 ? 2 : 1;  // bytes of a scale
+    extern __shared__ __align__(128) uint8_t dyn[];
+    __shared__ MvShared<P> sh;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int steps = mv_steps(a.K), G = a.K >> 5, SG = G >> a.group_shift, D = a.depth;
+    // dynamic shared memory: zeros, the ring of codes, that of scales, x [min(RP, R)][steps * 128] fp16, its scales
+    const int stage_bytes = MV_TILE * a.pitch, scales_at = 128 + D * stage_bytes;
+    const int xs_at = scales_at + a.scale_slots * a.scale_slot, xsc_at = xs_at + min(RP, a.R) * steps * 256;
+    if (tid < 4)
+        reinterpret_cast<uint4*>(dyn)[tid] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) {
+        for (int i = 0; i < D; i++) {
+            mbar_init(smem_u32(&sh.full[i]), 1);
+            mbar_init(smem_u32(&sh.done[i]), MV_WARPS);
+        }
+        sh.abort = 0;
+        fence_barrier_init();
+    }
+
+    pdl_wait();
+    pdl_trigger();
+
+    // the list of leaders: rows that open a pass over their matrix
+    int n_lead;
+    if (a.ids) {
+        int id = -1, rank = 0;
+        if (tid < a.R) {
+            id = a.ids[tid];
+            if (id < 0 || id >= a.n_mats)
+                id = -1;
+            sh.ids[tid] = id;
+        }
+        __syncthreads();
+        if (id >= 0)
+            for (int j = 0; j < tid; j++)
+                rank += sh.ids[j] == id;
+        if (tid < a.R)
+            sh.rank[tid] = id >= 0 ? rank : -1;
+        __syncthreads();
+        n_lead = 0;
+        for (int m0 = 0; m0 < a.R; m0 += 32) {  // every warp finds the same
+            const int m = m0 + lane;
+            const bool lead = m < a.R && sh.rank[m] >= 0 && sh.rank[m] % RP == 0;
+            const unsigned votes = __ballot_sync(0xffffffffu, lead);
+            if (lead)
+                sh.lead[n_lead + __popc(votes & ((1u << lane) - 1u))] = m;
+            n_lead += __popc(votes);
+        }
+    } else {
+        n_lead = (a.R + RP - 1) / RP;
+    }
+    __syncthreads();
+    const long long total = (long long)n_lead * a.n_tiles;  // fits an int (checked by the host)
+    const int i0 = (int)(total * blockIdx.x / gridDim.x), i1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
+    const int li0 = i0 / a.n_tiles, tile0 = i0 - li0 * a.n_tiles;
+
+    if (warp == MV_WARPS) {
+        // ---- feeds the ring, and stores the tiles that the others have summed ----
+        // A stage is free, and its tile's sums are complete, when the eight warps have arrived on `done`.
+        int l_left = i1 - i0, l_li = li0, l_tile = tile0, l_c0 = 0, l_stage = 0, l_slot = 0;
+        auto load = [&]() {
+            if (l_left <= 0)
+                return;
+            const size_t row0 = (size_t)(a.ids ? sh.ids[sh.lead[l_li]] : 0) * a.N + l_tile * MV_TILE;
+            const int rows = min(MV_TILE, a.N - l_tile * MV_TILE);
+            const int pieces = min(a.chunk_steps * 4, G - l_c0 * 4);  // of 16 bytes
+            const uint32_t full = smem_u32(&sh.full[l_stage]);
+            const uint8_t* s = static_cast<const uint8_t*>(a.scales) + row0 * SG * SB;
+            const int scales = l_c0 == 0 ? rows * SG * SB : 0, bulk = a.scale_bulk ? scales & ~15 : 0;
+            const int to = scales_at + l_slot * a.scale_slot;
+            if (bulk < scales) {  // what no bulk copy may take; a later tile's may be written over it, after these stores
+                for (int i = bulk + lane; i < scales; i += 32)
+                    dyn[to + i] = s[i];
+                fence_proxy_async_smem();
+            }
+            __syncwarp();
+            if (lane == 0)
+                mbar_expect_tx(full, rows * pieces * 16 + bulk);
+            __syncwarp();
+            if (a.chunk_steps == steps) {  // whole rows, as they lie
+                if (lane == 0)
+                    bulk_load(smem_u32(dyn) + 128 + l_stage * stage_bytes, a.codes + row0 * G * 16, rows * G * 16, full);
+            } else if (lane < rows)
+                bulk_load(smem_u32(dyn) + 128 + l_stage * stage_bytes + lane * a.pitch,
+                          a.codes + ((row0 + lane) * G + l_c0 * 4) * 16, pieces * 16, full);
+            if (lane == 31 && bulk)
+                bulk_load(smem_u32(dyn) + to, s, bulk, full);
+            l_stage = l_stage + 1 == D ? 0 : l_stage + 1;
+            l_c0 += a.chunk_steps;
+            if (l_c0 >= steps) {
+                l_c0 = 0;
+                l_left--;
+                l_slot = l_slot + 1 == a.scale_slots ? 0 : l_slot + 1;
+                if (++l_tile == a.n_tiles) {
+                    l_tile = 0;
+                    l_li++;
+                }
+            }
+        };
+        for (int i = 0; i < D; i++)
+            load();
+        int li = li0, tile = tile0, stage = 0, cur_lead = -1, cnt = 0, mat = 0;
+        uint32_t parity = 0;
+        bool ok = true;
+        for (int item = i0; item < i1; item++) {
+            if (li != cur_lead) {  // the rows of this pass
+                cur_lead = li;
+                __syncwarp();
+                if (a.ids) {
+                    const int first = sh.rank[sh.lead[li]];
+                    mat = sh.ids[sh.lead[li]];
+                    cnt = 0;
+                    for (int m0 = 0; m0 < a.R; m0 += 32) {
+                        const int m = m0 + lane;
+                        const bool in = m < a.R && sh.ids[m] == mat && sh.rank[m] >= first && sh.rank[m] < first + RP;
+                        if (in)
+                            sh.store_rows[sh.rank[m] - first] = m;
+                        cnt += __popc(__ballot_sync(0xffffffffu, in));
+                    }
+                } else {
+                    cnt = min(RP, a.R - li * RP);
+                    if (lane < cnt)
+                        sh.store_rows[lane] = li * RP + lane;
+                }
+                __syncwarp();
+            }
+            float bias[2];
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                const int n = tile * MV_TILE + g + 8 * half;
+                bias[half] = a.bias && n < a.N ? a.bias[(size_t)mat * a.N + n] : 0.f;
+            }
+            float2 v[P];
+            for (int c0 = 0; c0 < steps; c0 += a.chunk_steps) {
+                ok = ok && mbar_wait(smem_u32(&sh.done[stage]), parity, nullptr, 0, &sh.abort) &&
+                     *(volatile int*)&sh.abort == 0;
+                ok = __all_sync(0xffffffffu, ok);
+                if (c0 + a.chunk_steps >= steps) {
+                    // lane: row g of both halves, x row 2 p + t / 2 (the same in lanes t and t ^ 1); warps in order
+#pragma unroll
+                    for (int p = 0; p < P; p++) {
+                        v[p] = make_float2(0.f, 0.f);
+#pragma unroll
+                        for (int w = 0; w < MV_WARPS; w++) {
+                            const float2 r = sh.red[stage][w][p][lane >> 1];
+                            v[p].x += r.x;
+                            v[p].y += r.y;
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (ok)
+                    load();
+                if (++stage == D) {
+                    stage = 0;
+                    parity ^= 1;
+                }
+            }
+            const float poison = ok ? 0.f : __int_as_float(0x7FC00000);  // a wait that ran out leaves NaN
+#pragma unroll
+            for (int p = 0; p < P; p++) {
+                if (2 * p >= cnt)
+                    break;
+                const int c = 2 * p + (t >> 1);
+                const long long row = (long long)sh.store_rows[min(c, cnt - 1)] * a.out_stride;
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const int n = tile * MV_TILE + g + 8 * half;
+                    const float s = (half ? v[p].y : v[p].x) + bias[half] + poison;
+                    const float up_raw = __shfl_down_sync(0xffffffffu, s, 4);  // row g + 1
+                    if ((t & 1) == 0 && c < cnt && n < a.N) {
+                        if (!a.swiglu) {
+                            store_from_float(a.out, row + n, a.out_dtype, s);
+                        } else if ((g & 1) == 0) {
+                            const float gt = s > a.limit ? a.limit : s;  // comparisons that let NaN through
+                            const float up = up_raw > a.limit ? a.limit : up_raw < -a.limit ? -a.limit : up_raw;
+                            store_from_float(a.out, row + (n >> 1), a.out_dtype, gt / (1.f + expf(-a.alpha * gt)) * (up + 1.f));
+                        }
+                    }
+                }
+            }
+            if (++tile == a.n_tiles) {
+                tile = 0;
+                li++;
+            }
+        }
+        if (!ok)  // copies that are still on their way get a bounded time to land
+            for (int i = 0; i < D; i++) {
+                drain_wait(smem_u32(&sh.full[i]), 0);
+                drain_wait(smem_u32(&sh.full[i]), 1);
+            }
+        // rows without a matrix
+        if (a.ids) {
+            const int n_out = a.swiglu ? a.N >> 1 : a.N;
+            for (int m = 0; m < a.R; m++)
+                if (sh.ids[m] < 0)
+                    for (long long n = (long long)blockIdx.x * 32 + lane; n < n_out; n += (long long)gridDim.x * 32)
+                        store_from_float(a.out, m * a.out_stride + n, a.out_dtype, 0.f);
+        }
+        return;
+    }
+
+    // ---- computes ----
+    MvRun r{li0, 0, tile0, 0, 0, 0, 0};
+    for (int left = i1 - i0; left > 0; r.li++, r.tile = 0) {
+        // the rows of this pass, their x in fp16 and its scales
+        asm volatile("bar.sync 1, %0;" ::"n"(MV_THREADS) : "memory");  // nobody computes with the last ones
+        int cnt = 0;
+        if (a.ids) {
+            const int first = sh.rank[sh.lead[r.li]], mat = sh.ids[sh.lead[r.li]];
+            for (int m0 = 0; m0 < a.R; m0 += 32) {  // every warp counts, each stores the same
+                const int m = m0 + lane;
+                const bool in = m < a.R && sh.ids[m] == mat && sh.rank[m] >= first && sh.rank[m] < first + RP;
+                if (in)
+                    sh.rows[sh.rank[m] - first] = m;
+                cnt += __popc(__ballot_sync(0xffffffffu, in));
+            }
+        } else {
+            cnt = min(RP, a.R - r.li * RP);
+            if (lane < cnt)
+                sh.rows[lane] = r.li * RP + lane;
+        }
+        __syncwarp();
+        bool any = false;
+        for (int c = 0; c < cnt; c++)
+            any |= mv_load_x<INT4>(a, sh.rows[c] / a.rows_per_x, steps, G, reinterpret_cast<uint4*>(dyn + xs_at) + c * steps * 16,
+                                   reinterpret_cast<float*>(dyn + xsc_at) + c * steps * 4);
+        uint32_t far;
+        asm volatile("{\n\t.reg .pred p, q;\n\t"
+                     "setp.ne.u32 p, %1, 0;\n\t"
+                     "bar.red.or.pred q, 1, %2, p;\n\t"
+                     "selp.u32 %0, 1, 0, q;\n\t}"
+                     : "=r"(far)
+                     : "r"((uint32_t)any), "n"(MV_THREADS)
+                     : "memory");
+        const int n = min(left, a.n_tiles - r.tile);
+        left -= n;
+        r.cnt = cnt;
+        r.tile_end = r.tile + n;
+        if (__builtin_expect(far, 0)) {
+            mv_tiles<INT4, PAIRED, P, true>(a, sh, dyn, r);
+        } else {
+            mv_tiles<INT4, PAIRED, P, false>(a, sh, dyn, r);
         }
     }
 }

@@ -63,3 +63,117 @@ def test_group_sums_above_the_largest_value_still_order(E, G):
         kw = dict(score="sigmoid", bias=bias, n_groups=G, topk_groups=keep, group_top=2)
         r = pkg.route_logits(logits, k, **kw)
         _check_route(logits, k, r, **kw)
+
+
+# -- w4_matvec: x and scales of any size ----------------------------------------------
+
+
+def _wide_x(g, rows, K, lo, hi):
+    """bf16 values whose exponents are spread over lo..hi inside every group of 32."""
+    e = lo + (hi - lo) * torch.rand(rows, K, generator=g, device="cuda", dtype=torch.float64)
+    sign = torch.randint(0, 2, (rows, K), generator=g, device="cuda").double() * 2 - 1
+    return (sign * torch.exp2(e)).to(BF16)
+
+
+def _zero_codes(codes, where, fmt):
+    """Clears the weights of the columns `where` (bool [K])."""
+    zero = 8 if fmt == "int4" else 0
+    lo, hi = codes & 15, codes >> 4
+    lo[..., where[0::2]] = zero
+    hi[..., where[1::2]] = zero
+    return lo | hi << 4
+
+
+def test_matvec_a_small_value_beside_a_large_one():
+    """What is left of 2^k beside 1 where the weight of the large one is zero."""
+    codes = torch.zeros(16, 16, dtype=torch.uint8, device="cuda")
+    codes[:, 0] = 0x20  # 0 in column 0, 1.0 in column 1
+    scales = torch.full((16, 1), 127, dtype=torch.uint8, device="cuda")
+    x = torch.zeros(127, 32, dtype=BF16, device="cuda")
+    x[:, 0] = torch.exp2(torch.arange(1, 128, device="cuda").double()).to(BF16)
+    x[:, 1] = 1.6015625
+    assert (pkg.w4_matvec(x, codes, scales, dtype=F32) == 1.6015625).all()
+    x[:, 1] = -(2.0**-126)
+    assert (pkg.w4_matvec(x, codes, scales, dtype=F32) == -(2.0**-126)).all()
+
+
+@pytest.mark.parametrize("fmt,group", [("mxfp4", 32), ("int4", 32), ("int4", 128)])
+@pytest.mark.parametrize("N,K,M", [(17, 32, 1), (40, 416, 3), (12001, 160, 4), (48, 2880, 9), (300, 6144, 2), (33, 16384, 4)])
+@pytest.mark.parametrize("lo,hi", [(-60, 60), (-120, -40), (-126, 100)])
+def test_matvec_bf16_of_any_size_inside_a_group(fmt, group, N, K, M, lo, hi):
+    """Exponents spread inside every group, the largest values on weights of zero in some of the columns."""
+    if K % group:
+        K = -(-K // group) * group
+    g = _gen(N + K + M + lo)
+    codes, scales = _weights(g, (), N, K, fmt, group)
+    x = _wide_x(g, M, K, lo, hi)
+    # columns that are large in the first row have no weights: that row's result is what is left
+    large = x[0].double().abs() > 2.0 ** ((lo + hi) / 2 - 20)
+    codes = _zero_codes(codes, large, fmt)
+    x[-1, ::3] = 0
+    y = pkg.w4_matvec(x, codes, scales, dtype=F32)
+    _check_matvec(y, x.double(), codes, scales, None, group, None, 1)
+
+
+def test_matvec_mixed_rows_keep_their_bits():
+    """A row that spans many powers of two beside ordinary ones: each row as alone, whatever the batch and the ring."""
+    g = _gen(31)
+    for n, N, K in ((4, 3000, 544), (3, 100, 11264)):
+        codes, scales = _weights(g, (n,), N, K, "mxfp4", 32)
+        x = _randn(g, 12, K).to(BF16)
+        x[1] = _wide_x(g, 1, K, -90, 90)[0]
+        x[6, 64:] = _wide_x(g, 1, K, -90, 90)[0, 64:]
+        x[7] = 0
+        ids = torch.tensor([0, 1, 1, 0, 2, 1, 1, 1, 0, 1, 1, 1], dtype=torch.int32, device="cuda")
+        y = pkg.w4_matvec(x, codes, scales, ids=ids, dtype=F32)
+        _check_matvec(y, x.double(), codes, scales, None, 32, ids, 1)
+        for m in range(12):
+            e = int(ids[m])
+            assert torch.equal(y[m:m + 1], pkg.w4_matvec(x[m:m + 1], codes[e], scales[e], dtype=F32))
+
+
+@pytest.mark.parametrize("P", [1, 4])
+def test_matvec_large_x_times_small_scales(P):
+    """Products whose parts leave fp32 although they do not."""
+    g = _gen(13)
+    N, K = 80, 256
+    codes, scales = _weights(g, (), N, K, "mxfp4", 32)
+    x = (_randn(g, P, K).clamp(-3.9, 3.9).double() * 2.0**125).to(BF16)
+    for shift in (-60, -100):  # scales 2^(-8..-4) more
+        s = (scales.int() + shift).to(torch.uint8)
+        _check_matvec(pkg.w4_matvec(x, codes, s, dtype=F32), x.double(), codes, s, None, 32, None, 1)
+    x = (_randn(g, P, K).double() * 2.0**-127).to(BF16)  # the smallest are subnormal
+    for shift in (60, 130):
+        s = (scales.int() + shift).to(torch.uint8)
+        _check_matvec(pkg.w4_matvec(x, codes, s, dtype=F32), x.double(), codes, s, None, 32, None, 1)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "int4"])
+def test_matvec_every_x_scale_times_its_counterpart(fmt):
+    """e4m3 rows whose MX scale and weight scale are far apart and meet around 1; fp32 scales likewise."""
+    g = _gen(17)
+    K, R = 64, 255
+    q = _randn(g, R, K).to(torch.float8_e4m3fn)
+    sx = torch.arange(R, device="cuda").to(torch.uint8)
+    codes = torch.randint(0, 256, (R, 16, K // 2), generator=g, device="cuda", dtype=torch.uint8)
+    back = (254 - sx.int()).clamp(1, 254)
+    if fmt == "mxfp4":
+        scales = back.to(torch.uint8)[:, None, None].expand(R, 16, K // 32).contiguous()
+    else:
+        scales = torch.exp2(back.double() - 127).to(BF16)[:, None, None].expand(R, 16, K // 32).contiguous()
+    ids = torch.arange(R, dtype=torch.int32, device="cuda")
+    x64 = q.double() * torch.exp2(sx.double() - 127)[:, None]
+    y = pkg.w4_matvec(q, codes, scales, x_scales=sx[:, None].expand(R, K // 32).contiguous(), ids=ids, dtype=F32)
+    _check_matvec(y, x64, codes, scales, None, 32, ids, 1)
+    row = torch.exp2(sx.double() - 127).float()[:, None].contiguous()
+    y = pkg.w4_matvec(q, codes, scales, x_scales=row, ids=ids, dtype=F32)
+    _check_matvec(y, x64, codes, scales, None, 32, ids, 1)
+
+
+def test_matvec_x_scales_of_zero_infinity_and_nan():
+    codes = torch.full((16, 32), 0x22, dtype=torch.uint8, device="cuda")  # 1.0 everywhere
+    scales = torch.full((16, 2), 127, dtype=torch.uint8, device="cuda")
+    q = torch.ones(4, 64, device="cuda").to(torch.float8_e4m3fn)
+    s = torch.tensor([[0.0, 1.0], [math.inf, 1.0], [math.nan, 1.0], [-2.0, 0.5]], device="cuda")
+    y = pkg.w4_matvec(q, codes, scales, x_scales=s, dtype=F32)
+    assert (y[0] == 32).all() and (y[1] == math.inf).all() and y[2].isnan().all() and (y[3] == -48).all()
