@@ -4,6 +4,9 @@
 block for tensors of the caller's own (include/moe_b200.h): they take no handle and keep
 nothing.  Results go where the caller says or into new tensors; the calls are asynchronous
 on ``stream`` (a ``torch.cuda.Stream``; by default the current stream of the tensors' device).
+A call on a ``stream`` of its own waits for nothing on the stream that made its inputs: order the two
+with ``wait_stream``, as for any torch operator.  Inputs may be dropped after the call: their memory is
+kept until ``stream`` has passed it.
 A wrong argument raises ``ValueError`` here or ``capi.MoEError`` with the library's text.
 """
 from __future__ import annotations
@@ -79,10 +82,15 @@ def _device(t):
 
 
 def _on(stream, fn, x, *args, **kw):
-    """The call with `stream` as the current one: new results come from that stream's memory."""
+    """The call with `stream` as the current one: new results come from that stream's memory, and the memory of the
+    tensors of the caller's is not handed out again before `stream` has passed the call."""
     _need(stream.device == x.device, "stream: needs the device of the tensors")
     with torch.cuda.stream(stream):
-        return fn(x, *args, **kw)
+        result = fn(x, *args, **kw)
+    for t in (x, *args, *kw.values()):
+        if isinstance(t, torch.Tensor):
+            t.record_stream(stream)
+    return result
 
 
 def _call(name, dev, args):

@@ -177,3 +177,35 @@ def test_matvec_x_scales_of_zero_infinity_and_nan():
     s = torch.tensor([[0.0, 1.0], [math.inf, 1.0], [math.nan, 1.0], [-2.0, 0.5]], device="cuda")
     y = pkg.w4_matvec(q, codes, scales, x_scales=s, dtype=F32)
     assert (y[0] == 32).all() and (y[1] == math.inf).all() and y[2].isnan().all() and (y[3] == -48).all()
+
+
+# -- calls beside other work ---------------------------------------------------------------
+
+
+def test_inputs_of_a_call_on_another_stream_may_be_dropped():
+    """The memory of an input that the caller lets go is not handed out before the call on the other stream has read it."""
+    g = _gen(23)
+    s = torch.cuda.Stream()
+    T, H, E = 64, 4096, 128
+    w = torch.ones(H, device="cuda")
+    codes, scales = _weights(g, (), 512, H, "mxfp4", 32)
+    x, logits = _randn(g, T, H), _randn(g, T, E)
+    xb = x.to(BF16)
+    want = pkg.add_rmsnorm(x, w, x, quant="mx"), pkg.route_logits(logits, 4), (pkg.w4_matvec(xb, codes, scales),)
+    calls = [lambda: pkg.add_rmsnorm(x.clone(), w, x.clone(), quant="mx", stream=s),
+             lambda: pkg.route_logits(logits.clone(), 4, stream=s),
+             lambda: (pkg.w4_matvec(xb.clone(), codes, scales, stream=s),)]
+    for call, ref_out in zip(calls, want):
+        for t in (x, xb, logits):
+            t.clone()  # the sizes that the call's temporaries have are in the allocator's lists
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(20_000_000)  # about 10 ms
+        got = call()
+        s_busy = not s.query()
+        trash = [torch.full_like(t, 7.0) for t in (x, x, xb, logits) for _ in range(2)]
+        torch.cuda.synchronize()
+        assert s_busy, "the call has to be waiting while its inputs' memory could be reused"
+        for a, b in zip(got, ref_out):
+            assert (a is None and b is None) or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        del trash
