@@ -28,6 +28,14 @@ moe_b200_status refuse(moe_b200_status st, const char* fmt, ...) {
 
 #define INVALID(...) return refuse(MOE_B200_ERR_INVALID, __VA_ARGS__)
 
+// A failed CUDA call leaves its error behind, and a later call of the library that asks for the last one would report it.
+moe_b200_status cuda_status(const char* what, cudaError_t e) {
+    if (e == cudaSuccess)
+        return MOE_B200_OK;
+    cudaGetLastError();
+    return refuse(MOE_B200_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
 // Device and SM count of the calling thread's current device.
 moe_b200_status current_device(int* dev, int* sms) {
     static std::atomic<int> cache[MAX_DEVICES];
@@ -37,9 +45,8 @@ moe_b200_status current_device(int* dev, int* sms) {
     }
     int n = *dev < MAX_DEVICES ? cache[*dev].load(std::memory_order_relaxed) : 0;
     if (n == 0) {
-        cudaError_t e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, *dev);
-        if (e != cudaSuccess)
-            return refuse(MOE_B200_ERR_CUDA, "cudaDeviceGetAttribute: %s", cudaGetErrorString(e));
+        if (moe_b200_status st = cuda_status("cudaDeviceGetAttribute", cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, *dev)))
+            return st;
         if (*dev < MAX_DEVICES)
             cache[*dev].store(n, std::memory_order_relaxed);
     }
@@ -65,10 +72,6 @@ cudaError_t launch(void (*kernel)(Params...), unsigned grid, dim3 block, size_t 
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
-moe_b200_status launched(const char* what, cudaError_t e) {
-    return e == cudaSuccess ? MOE_B200_OK : refuse(MOE_B200_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
 bool is_float_type(int dtype) {
@@ -149,7 +152,7 @@ moe_b200_status moe_b200_add_rmsnorm(const moe_b200_add_rmsnorm_args* args, moe_
     const int together = threads == 32 && n_rows >= 8 * sms ? 8 : 1;  // rows per block; 16384 x 64: 5.7 us, one 10.3
     const unsigned grid = (unsigned)(((long long)n_rows + together - 1) / together);
     a.early = grid <= 2u * sms;
-    return launched("moe_b200_add_rmsnorm", launch(kernel, grid, dim3(threads, together), 0, st, a));
+    return cuda_status("moe_b200_add_rmsnorm", launch(kernel, grid, dim3(threads, together), 0, st, a));
 }
 
 moe_b200_status moe_b200_route_logits(const moe_b200_route_logits_args* args, moe_b200_stream stream) {
@@ -190,7 +193,7 @@ moe_b200_status moe_b200_route_logits(const moe_b200_route_logits_args* args, mo
         return st;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (n_tokens == 0)
-        return launched("moe_b200_route_logits: counts", cudaMemsetAsync(expert_counts, 0, sizeof(int) * (size_t)E, st));
+        return cuda_status("moe_b200_route_logits: counts", cudaMemsetAsync(expert_counts, 0, sizeof(int) * (size_t)E, st));
     const int nt = E <= 32 ? 1 : E <= 64 ? 2 : E <= 128 ? 4 : E <= 256 ? 8 : 16;
     int lane_shift = 5;
     while (n_groups << lane_shift > 32)
@@ -216,7 +219,7 @@ moe_b200_status moe_b200_route_logits(const moe_b200_route_logits_args* args, mo
         const int n = n_tokens * K, blocks = (n + 2047) / 2048;
         e = launch(route_counts_kernel, blocks < sms ? blocks : sms, 256, 0, st, (const int*)topk_i, n, E, expert_counts);
     }
-    return launched("moe_b200_route_logits", e);
+    return cuda_status("moe_b200_route_logits", e);
 }
 
 moe_b200_status moe_b200_w4_matvec(const moe_b200_w4_matvec_args* args, moe_b200_stream stream) {
@@ -359,11 +362,11 @@ moe_b200_status moe_b200_w4_matvec(const moe_b200_w4_matvec_args* args, moe_b200
         cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              (int)(MV_SM_SMEM - 1024 - mv_static_bytes(pairs)));
         if (e != cudaSuccess)
-            return launched("moe_b200_w4_matvec: shared memory", e);
+            return cuda_status("moe_b200_w4_matvec: shared memory", e);
     }
     const long long passes = ids ? n_rows : (n_rows + 2 * pairs - 1) / (2 * pairs);
     const long long items = passes * a.n_tiles, most = (long long)blocks * sms;
-    return launched("moe_b200_w4_matvec", launch(kernel, (unsigned)(items < most ? items : most), MV_BLOCK, smem, st, a));
+    return cuda_status("moe_b200_w4_matvec", launch(kernel, (unsigned)(items < most ? items : most), MV_BLOCK, smem, st, a));
 }
 
 }  // extern "C"

@@ -209,3 +209,41 @@ def test_inputs_of_a_call_on_another_stream_may_be_dropped():
         for a, b in zip(got, ref_out):
             assert (a is None and b is None) or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
         del trash
+
+
+def test_a_refused_launch_leaves_no_error_behind():
+    """CUDA refuses work on the legacy stream while an ordinary stream of the thread is being captured.  The call
+    says so, and the next call of the library starts from a clean state."""
+    from cuda.bindings import runtime as rt
+
+    from gpt_oss_amd_b200 import capi
+
+    x, w = torch.ones(4, 64, device="cuda"), torch.ones(64, device="cuda")
+    y = torch.empty(4, 64, device="cuda")
+    logits, ti, tw = torch.ones(4, 8, device="cuda"), torch.empty(4, 2, dtype=torch.int32, device="cuda"), torch.empty(4, 2, device="cuda")
+    q, codes, scales = x.to(BF16), torch.zeros(16, 32, dtype=torch.uint8, device="cuda"), torch.zeros(16, 2, dtype=torch.uint8, device="cuda")
+    out = torch.empty(4, 16, device="cuda")
+    blocks = torch.zeros(4, 2, 16, dtype=torch.uint8, device="cuda")
+    sc = torch.full((4, 2), 127, dtype=torch.uint8, device="cuda")
+    un = torch.empty(4, 64, dtype=torch.int16, device="cuda")
+    L = capi.lib()
+    norm = capi.packer(capi.AddRmsnormArgs)(4, 64, x.data_ptr(), 0, 64, 0, 0, 0, 0, 0, w.data_ptr(), 0, 1e-5, y.data_ptr(), 0, 64, 0, 0, 0, 0)
+    route = capi.packer(capi.RouteLogitsArgs)(4, 8, 2, logits.data_ptr(), 0, 8, 0, 0, 1, 1, 1, 1, 1.0, ti.data_ptr(), tw.data_ptr(), 0)
+    matvec = capi.packer(capi.W4MatvecArgs)(0, 32, 1, 16, 64, codes.data_ptr(), scales.data_ptr(), 0, q.data_ptr(), 1, 64, 0, 0, 4, 1, 0,
+                                            0, 0.0, 0.0, out.data_ptr(), 0, 16)
+    torch.cuda.synchronize()
+    for fn, args in ((L.moe_b200_add_rmsnorm, norm), (L.moe_b200_route_logits, route), (L.moe_b200_w4_matvec, matvec)):
+        err, stream = rt.cudaStreamCreate()
+        assert err == rt.cudaError_t.cudaSuccess
+        err, = rt.cudaStreamBeginCapture(stream, rt.cudaStreamCaptureMode.cudaStreamCaptureModeThreadLocal)
+        assert err == rt.cudaError_t.cudaSuccess
+        status = fn(args, None)
+        text = L.moe_b200_last_error(None)
+        rt.cudaStreamEndCapture(stream)
+        rt.cudaGetLastError()
+        rt.cudaStreamDestroy(stream)
+        assert status == capi.ERR_CUDA and b"captur" in text, (status, text)
+        assert fn(args, None) == capi.OK
+        status = L.moe_b200_mxfp4_unpack(blocks.data_ptr(), sc.data_ptr(), 4, 2, un.data_ptr(), None)
+        assert status == capi.OK, L.moe_b200_last_error(None)
+    torch.cuda.synchronize()
