@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <cstdlib>
+
 namespace moe {
 
 // ---------------------------------------------------------------------------
@@ -151,14 +153,22 @@ __host__ __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b -
 // does its own set-up (shared-memory init, barriers, tensor-memory allocation) and calls
 // pdl_wait() before it touches anything that kernel wrote -- the wait returns when the
 // whole previous grid has completed and its memory is visible.  pdl_trigger() lets the
-// NEXT kernel start its own set-up early.  Both are no-ops in a kernel launched the
-// ordinary way.  Every kernel of the forward path calls both, and writes nothing to global
+// NEXT kernel start its own set-up early, if that one was launched with the attribute.  pdl_wait()
+// returns at once in a kernel launched the ordinary way.  Every kernel of the forward path calls both, and writes nothing to global
 // memory before the wait.
 // The kernels from the permute on trigger AFTER their wait.  So when the kernel behind one of
 // them starts, every kernel before that one has completed: the down GEMM may read the
 // plan, and the combine the routing, before their own wait -- through ld_l2() only.
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// MOE_B200_NO_PDL=1 in the environment switches the attribute off for the kernels of a small-batch
+// single-GPU call and for the stand-alone operators, the two that have it (a debugging aid: all
+// kernels of the library then run strictly one after the other).
+inline bool pdl_enabled() {
+    static const bool on = std::getenv("MOE_B200_NO_PDL") == nullptr;
+    return on;
+}
 
 // A load before this kernel's own pdl_wait(), of what a kernel two or more back stored.
 // Guaranteed: that kernel has completed (above), and the kernel between the two waited for it,

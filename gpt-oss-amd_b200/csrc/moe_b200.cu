@@ -159,15 +159,6 @@ bool word_store_ok(const void* p, int device) {
     return word_store_ok(p, a, device);
 }
 
-// Programmatic dependent launch (pdl_wait / pdl_trigger in common.cuh) for the kernels
-// of a small-batch single-GPU call: each may start its set-up while the kernel before
-// it drains.  MOE_B200_NO_PDL=1 in the environment switches it off (a debugging aid:
-// the kernels then run strictly one after the other, as on every other path).
-bool pdl_enabled() {
-    static const bool on = std::getenv("MOE_B200_NO_PDL") == nullptr;
-    return on;
-}
-
 // `cluster` CTAs per thread-block cluster (1: none).
 template <typename... KArgs, typename... Args>
 cudaError_t launch_clusters(int cluster, bool pdl, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,

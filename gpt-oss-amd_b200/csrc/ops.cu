@@ -54,7 +54,7 @@ moe_b200_status current_device(int* dev, int* sms) {
     return MOE_B200_OK;
 }
 
-// Launches as a programmatic dependent of the kernel in front: every kernel here waits for its end before it touches
+// Launches as a programmatic dependent of the kernel in front (unless pdl_enabled() says no): every kernel here waits for its end before it touches
 // global memory, and then lets the next one's blocks come to the SMs (`early`) if it has two blocks per SM at most.
 // Behind larger grids they would crowd where room is first: us per call in a replayed chain, launched the ordinary way,
 // always early, by this rule: add_rmsnorm 1 x 2880 2.2, 2.0, 2.0; 777 x 2047 6.4, 7.6, 6.3; route_logits 1 x 128 2.7, 2.2,
@@ -70,7 +70,7 @@ cudaError_t launch(void (*kernel)(Params...), unsigned grid, dim3 block, size_t 
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = moe::pdl_enabled() ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 

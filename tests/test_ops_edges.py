@@ -247,3 +247,47 @@ def test_a_refused_launch_leaves_no_error_behind():
         status = L.moe_b200_mxfp4_unpack(blocks.data_ptr(), sc.data_ptr(), 4, 2, un.data_ptr(), None)
         assert status == capi.OK, L.moe_b200_last_error(None)
     torch.cuda.synchronize()
+
+
+def _three_calls():
+    x = torch.ones(4, 64, device="cuda", dtype=BF16)
+    n = pkg.add_rmsnorm(x, torch.ones(64, device="cuda"))
+    r = pkg.route_logits(n.y, 4, counts=True)
+    codes, scales = torch.zeros(16, 32, dtype=torch.uint8, device="cuda"), torch.zeros(16, 2, dtype=torch.uint8, device="cuda")
+    return pkg.w4_matvec(n.y, codes, scales), r
+
+
+_EDGES = """
+import torch
+import sys
+sys.path.insert(0, "tests")
+from cuda.bindings import runtime as rt
+from test_ops_edges import _three_calls
+_three_calls()
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph(keep_graph=True)
+with torch.cuda.graph(g):
+    _three_calls()
+raw = rt.cudaGraph_t(init_value=g.raw_cuda_graph())
+err, _, _, _, n = rt.cudaGraphGetEdges_v2(raw, 0)
+err, _, _, data, n = rt.cudaGraphGetEdges_v2(raw, n)
+assert err == rt.cudaError_t.cudaSuccess
+print("programmatic", sum(int(d.type) == int(rt.cudaGraphDependencyType.cudaGraphDependencyTypeProgrammatic) for d in data))
+"""
+
+
+@pytest.mark.parametrize("off", [False, True])
+def test_the_switch_for_dependent_launches_reaches_the_operators(off):
+    """MOE_B200_NO_PDL: every kernel behind the end of the one in front."""
+    import os
+    import subprocess
+    import sys
+
+    env = {k: v for k, v in os.environ.items() if k != "MOE_B200_NO_PDL"}
+    if off:
+        env["MOE_B200_NO_PDL"] = "1"
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _EDGES], cwd=root, env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    n = int(r.stdout.split("programmatic")[1])
+    assert n == 0 if off else n >= 2
