@@ -113,7 +113,7 @@ moe_b200_status fail(moe_b200_handle h, moe_b200_status st, const std::string& m
     if (h)
         h->err = msg;
     else
-        snprintf(moe::thread_error(), moe::THREAD_ERROR_BYTES, "%s", msg.c_str());
+        moe::set_common_error(msg.c_str());
     return st;
 }
 
@@ -1514,7 +1514,7 @@ void moe_b200_batcher_stats(moe_b200_batcher b, long long* steps, long long* row
 size_t moe_b200_device_bytes(moe_b200_handle h) { return h ? h->device_bytes : 0; }
 
 const char* moe_b200_last_error(moe_b200_handle h) {
-    return h ? h->err.c_str() : moe::thread_error();
+    return h ? h->err.c_str() : moe::last_error();
 }
 
 moe_b200_status moe_b200_device_status(moe_b200_handle h, int* status_word) {

@@ -19,10 +19,12 @@ constexpr int MAX_DEVICES = 64;
 constexpr size_t MV_SM_SMEM = 228 * 1024;  // of an SM
 
 moe_b200_status refuse(moe_b200_status st, const char* fmt, ...) {
+    char text[moe::ERROR_BYTES];
     va_list ap;
     va_start(ap, fmt);
-    vsnprintf(moe::thread_error(), moe::THREAD_ERROR_BYTES, fmt, ap);
+    vsnprintf(text, sizeof(text), fmt, ap);
     va_end(ap);
+    moe::set_thread_error(text);
     return st;
 }
 

@@ -275,9 +275,10 @@ void moe_b200_batcher_stats(moe_b200_batcher b, long long* steps, long long* row
 
 /* Bytes of device memory the handle holds (weights + workspace). */
 size_t moe_b200_device_bytes(moe_b200_handle h);
-/* Text of the last error on this handle or, when h is NULL, of the calling
- * thread's last failed call that has no handle (create and the stand-alone
- * functions).  Never NULL. */
+/* Text of the last error on this handle or, when h is NULL, of the last failed
+ * call that has no handle: of create and the functions around it in any thread, of
+ * the stand-alone operators in the calling one.  Never NULL; with NULL valid until
+ * the thread's next call. */
 const char* moe_b200_last_error(moe_b200_handle h);
 /* Reads AND CLEARS the device status word (synchronises the device): 0 = no
  * kernel has reported a problem since the last read; otherwise the code of the
