@@ -249,6 +249,46 @@ def test_a_refused_launch_leaves_no_error_behind():
     torch.cuda.synchronize()
 
 
+def test_branches_of_a_captured_graph_join():
+    """Two operators on streams of their own, and one behind both, behind a copy and in front of everything: captured
+    and replayed on new inputs."""
+    g = _gen(41)
+    T, H, E, K = 8, 576, 32, 4
+    w = 1 + 0.1 * _randn(g, H)
+    codes, scales = _weights(g, (E,), 300, H, "mxfp4", 32)
+    x, logits = _randn(g, T, H), _randn(g, T, E)
+    keep = torch.empty(T * K, 300, device="cuda")
+
+    def step(main, side):
+        if side is not main:
+            side.wait_stream(main)
+        with torch.cuda.stream(side):
+            r = pkg.route_logits(logits, K, counts=True)
+        n = pkg.add_rmsnorm(x, w, quant="mx")
+        if side is not main:
+            main.wait_stream(side)
+        y = pkg.w4_matvec(n.q, codes, scales, x_scales=n.q_scales, ids=r.topk_i.view(-1), rows_per_x=K, dtype=F32)
+        keep.copy_(y)
+        z = pkg.add_rmsnorm(keep, torch.ones(300, device="cuda"), keep, dtype=F32)
+        return r.topk_i, r.counts, n.y, y, z.y
+
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+    main.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(main):
+        step(main, side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=main):
+        got = step(main, side)
+    for _ in range(5):
+        x.normal_(generator=g)
+        logits.normal_(generator=g)
+        graph.replay()
+        s = torch.cuda.current_stream()
+        for a, b in zip(got, step(s, s)):
+            assert torch.equal(a, b)
+
+
 def _three_calls():
     x = torch.ones(4, 64, device="cuda", dtype=BF16)
     n = pkg.add_rmsnorm(x, torch.ones(64, device="cuda"))
