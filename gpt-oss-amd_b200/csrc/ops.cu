@@ -1,6 +1,7 @@
 // Host side of the stand-alone operators of include/moe_b200.h: argument checks and launches.
 // They need no handle, allocate nothing and keep nothing between calls.
 #include <cuda_runtime.h>
+#include <float.h>
 
 #include <atomic>
 #include <cstdarg>
@@ -102,7 +103,7 @@ moe_b200_status moe_b200_add_rmsnorm(const moe_b200_add_rmsnorm_args* args, moe_
     if (!is_float_type(x_dtype) || !is_float_type(weight_dtype) || (residual && !is_float_type(residual_dtype)) ||
         (y && !is_float_type(y_dtype)))
         INVALID("moe_b200_add_rmsnorm: x, residual, weight and y are f32, bf16 or f16");
-    if (!(eps >= 0.f) || eps > 3.0e38f)
+    if (!(eps >= 0.f && eps <= FLT_MAX))
         INVALID("moe_b200_add_rmsnorm: eps must be finite and not negative");
     int group = 0, mx = 0, n_scales = 1;
     if (q) {
@@ -179,7 +180,7 @@ moe_b200_status moe_b200_route_logits(const moe_b200_route_logits_args* args, mo
         INVALID("moe_b200_route_logits: a group is scored by its best or its two best experts");
     if ((long long)topk_groups * (E / n_groups) < K)
         INVALID("moe_b200_route_logits: the groups kept hold fewer than experts_per_token experts");
-    if (!(scale > -3.0e38f && scale < 3.0e38f))
+    if (!(scale >= -FLT_MAX && scale <= FLT_MAX))
         INVALID("moe_b200_route_logits: scale must be finite");
     if (n_tokens > 0 && (!logits || !topk_i || !topk_w))
         INVALID("moe_b200_route_logits: null pointer");
