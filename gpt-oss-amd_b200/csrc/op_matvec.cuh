@@ -178,33 +178,38 @@ __device__ __forceinline__ float mv_x_scale(const MatvecArgs& a, long long xr, i
     return a.xs_mx ? e8m0_to_float(static_cast<const uint8_t*>(a.x_scales)[at]) : static_cast<const float*>(a.x_scales)[at];
 }
 
-// bf16: exponent field of a group's largest value (14 at least) from its magnitude bits, and what is far.
-__device__ __forceinline__ uint32_t mv_top_exponent(uint32_t top) { return max(top >> 23, 14u); }
-__device__ __forceinline__ bool mv_far_group(uint32_t top) {  // the x scale 2^(ex - 141) is out of its range
-    return top != 0 && (mv_top_exponent(top) < 41u || mv_top_exponent(top) > 244u);
+// Maxima of two 16-bit lanes.
+__device__ __forceinline__ uint32_t mv_max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
 }
-__device__ __forceinline__ bool mv_far_value(uint32_t bits, uint32_t top) {
-    return (bits & 0x7FFFFFFFu) != 0 && ((bits >> 23) & 255u) + 31u < mv_top_exponent(top);
-}
-__device__ __forceinline__ bool mv_far_scale(float sc) { return !(sc == 0.f || (fabsf(sc) >= 0x1p-100f && fabsf(sc) <= 0x1p103f)); }
 
-// Largest magnitude of a group, eight values in each lane of a quad, as bits; `far`: something in it is far.
-__device__ __forceinline__ uint32_t mv_top(const uint32_t (&h)[4], int tid, bool& far) {
-    uint32_t most = 0, least = 0;  // the smallest but zero, less one, as its complement: both are maxima, of 16-bit lanes
+// Magnitudes of a group of bf16, eight values in each lane of a quad: the largest in the low half of the result, 2^16
+// less the smallest but zero in the high half (0: all are), so that both are maxima.
+__device__ __forceinline__ uint32_t mv_span(const uint32_t (&h)[4], int tid) {
+    uint32_t most = 0, least = 0;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         const uint32_t v = h[e] & 0x7FFF7FFFu;
-        most = __vmaxu2(most, v);
-        least = __vmaxu2(least, ~__vsub2(v, 0x00010001u));
+        most = mv_max2(most, v);
+        least = mv_max2(least, (0x80008000u - v) ^ 0x80008000u);  // 0 stays 0
     }
-    most = __vmaxu2(__byte_perm(most, least, 0x5410), __byte_perm(most, least, 0x7632));
+    most = mv_max2(__byte_perm(most, least, 0x5410), __byte_perm(most, least, 0x7632));
     const unsigned quad = 0xFu << (tid & 28);
-    most = __vmaxu2(most, __shfl_xor_sync(quad, most, 1));
-    most = __vmaxu2(most, __shfl_xor_sync(quad, most, 2));
-    const uint32_t top = most << 16;
-    far = mv_far_group(top) || mv_far_value((~most & 0xFFFF0000u) + 0x10000u, top);
-    return top;
+    most = mv_max2(most, __shfl_xor_sync(quad, most, 1));
+    return mv_max2(most, __shfl_xor_sync(quad, most, 2));
 }
+
+// What is far.  A group of bf16 by the exponent field of its largest value, which gives the x scale 2^(field - 141); a value
+// of a group that is not; a group of e4m3.
+__device__ __forceinline__ uint32_t mv_top(uint32_t span) { return (span & 0xFFFFu) >> 7; }
+__device__ __forceinline__ bool mv_far_group(uint32_t span) { return (span & 0xFFFFu) != 0 && mv_top(span) - 41u > 244u - 41u; }
+__device__ __forceinline__ bool mv_far_value(uint32_t bits16, uint32_t span) {
+    const uint32_t v = bits16 & 0x7FFFu;
+    return v != 0 && (v >> 7) + 31u < mv_top(span);
+}
+__device__ __forceinline__ bool mv_far_scale(float sc) { return !(sc == 0.f || (fabsf(sc) >= 0x1p-100f && fabsf(sc) <= 0x1p103f)); }
 
 // One row of x in fp16 and the scale of each of its groups, by all threads of the block.  Returns whether this thread
 // saw something far.
@@ -240,16 +245,25 @@ __device__ __forceinline__ bool mv_load_x(const MatvecArgs& a, long long xr, int
             }
         }
         if (a.x_dtype == MOE_B200_DTYPE_BF16) {
-            const uint32_t m = mv_top(h, tid, is_far);
-            const bool whole = mv_far_group(m);
-            if (is_far)
+            const uint32_t span = mv_span(h, tid);
+            uint32_t ex = mv_top(span);
+            // a group to look at: the largest value is out of range or zero, or 31 * 128 codes and more above the smallest
+            if (ex - 41u > 244u - 41u || (span & 0xFFFFu) + (span >> 16) > 0x10000u + 31u * 128u) {
+                if (ex - 41u > 244u - 41u) {
+                    is_far = mv_far_group(span);
+                    h[0] = h[1] = h[2] = h[3] = 0;
+                    ex = 127;
+                } else {
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    h[e] &= (whole || mv_far_value(h[e] << 16, m) ? 0u : 0x0000FFFFu) |
-                            (whole || mv_far_value(h[e] & 0xFFFF0000u, m) ? 0u : 0xFFFF0000u);
-            const uint32_t ex = mv_top_exponent(m);
+                    for (int e = 0; e < 4; e++) {
+                        const bool lo = mv_far_value(h[e], span), hi = mv_far_value(h[e] >> 16, span);
+                        h[e] &= (lo ? 0u : 0x0000FFFFu) | (hi ? 0u : 0xFFFF0000u);
+                        is_far = is_far || lo || hi;
+                    }
+                }
+            }
             const float up = __uint_as_float((268u - ex) << 23);  // 2^(141 - ex)
-            sc = grp < G && !whole ? __uint_as_float(max((ex - 14u) << 23, 0x00400000u)) : 0.f;
+            sc = __uint_as_float((ex - 14u) << 23);
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 h[e] = floats_to_half2(__uint_as_float(h[e] << 16) * up, __uint_as_float(h[e] & 0xFFFF0000u) * up, MOE_B200_DTYPE_F16);
@@ -288,9 +302,9 @@ __device__ __forceinline__ unsigned long long mv_far_groups(const MatvecArgs& a,
                 far = mv_far_scale(mv_x_scale(a, xr, grp));
             }
         }
-        bool far16;
-        mv_top(h, lane, far16);
-        const unsigned votes = __ballot_sync(0xffffffffu, far || far16);
+        const uint32_t span = mv_span(h, lane);
+        far = far || mv_far_group(span) || (span != 0 && mv_far_value(0x10000u - (span >> 16), span));
+        const unsigned votes = __ballot_sync(0xffffffffu, far);
 #pragma unroll
         for (int q = 0; q < 8; q++)
             all |= (unsigned long long)(votes >> (4 * q) & 1) << (at + q);
@@ -324,21 +338,20 @@ __device__ __forceinline__ float2 mv_far(const MatvecArgs& a, int mat, int n, lo
         uint32_t w0 = *reinterpret_cast<const uint32_t*>(a.codes + (row0 * G + grp) * 16 + t * 4);
         uint32_t w1 = *reinterpret_cast<const uint32_t*>(a.codes + (row1 * G + grp) * 16 + t * 4);
         const float s0 = scale(row0 * SG + (grp >> a.group_shift)), s1 = scale(row1 * SG + (grp >> a.group_shift));
-        uint32_t top = 0;
-        bool whole = true;
+        uint32_t span = 0;
         if (bf16) {
             const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + col);
             const uint32_t h[4] = {v.x, v.y, v.z, v.w};
-            top = mv_top(h, lane, whole);
-            whole = mv_far_group(top);
+            span = mv_span(h, lane);
         }
+        const bool whole = mv_far_group(span);
         double d0 = 0.0, d1 = 0.0;
 #pragma unroll 1
         for (int i = 0; i < 8; i++) {
             float x;
             if (bf16) {
-                const uint32_t bits = (uint32_t)static_cast<const uint16_t*>(a.x)[col + i] << 16;
-                x = whole || mv_far_value(bits, top) ? __uint_as_float(bits) : 0.f;
+                const uint32_t bits = static_cast<const uint16_t*>(a.x)[col + i];
+                x = whole || mv_far_value(bits, span) ? __uint_as_float(bits << 16) : 0.f;
             } else {
                 __nv_fp8_e4m3 v;
                 v.__x = static_cast<const uint8_t*>(a.x)[col + i];
