@@ -31,10 +31,11 @@
 //
 // Measured (201088 x 2880, mxfp4, one row: 308 MB, 48 us at the HBM rate).  Loads into registers, 8 rows x 64
 // bytes per instruction: 82 us with 32 warps per SM; a ring per warp filled by cp.async in the same
-// pattern: 72; a bulk copy per row: 81; one bulk copy per tile: 63.  Now 139 instructions per warp and step
-// (56 of them decoding) at 2.4 per clock pace it: 61 clocks per step and SM against 44 at the HBM rate. int4
-// decodes in 9 operations per 8 codes instead of 7: 83 us; a second pair of x rows adds 8 MMAs and
-// their x to a step: 104 us.  Four pairs per pass were slower than two passes (230 against 2 x 88 us).
+// pattern: 72; a bulk copy per row: 81; one bulk copy per tile: 62.5.  Now 132 instructions per warp and step
+// (56 of them decoding) at 2.2 per clock pace it: 60 clocks per step and SM against 44 at the HBM rate.  int4
+// decodes in 9 operations per 8 codes instead of 7: 81 us; a second pair of x rows adds 8 MMAs and
+// their x to a step: 86 us for three rows in mxfp4, 101 in int4.  Four pairs per pass were slower than two passes (230 us
+// against 164).
 #pragma once
 #include "common.cuh"
 #include "op_types.cuh"
@@ -88,8 +89,8 @@ __host__ __device__ constexpr int mv_steps(int K) { return (K + 127) / 128; }
 template <bool INT4>
 __device__ __forceinline__ void mv_decode(uint32_t w, uint32_t (&o)[4]) {
     if (INT4) {  // code - 8; pairs of columns (0, 4), (1, 5), (2, 6), (3, 7)
-        // 1024 | code, and 1024 + 16 code in the upper nibbles: one three-input operation each, the magic number
-        // kept in a register
+        // 1024 | code, and 1024 + 16 code in the upper nibbles, as is widely done: four bits put into the last ones of
+        // fp16's 1024 are added to it.  One three-input operation each, the 1024 kept in a register.
         uint32_t magic;
         asm("mov.b32 %0, 0x64006400;" : "=r"(magic));
         const __half2 sub = __floats2half2_rn(-1032.f, -1032.f), sub16 = __floats2half2_rn(-72.f, -72.f);
@@ -388,8 +389,8 @@ struct MvRun {
 };
 
 // The sums of the tiles of a pass.  FAR: something of its x is far.  Two instances: one with a test at the end of a tile
-// took 66 us for the vocabulary (one row, mxfp4), this takes 62.5; with one far value in x 142, with one in each of its
-// 90 groups 1200.
+// took 66 us for the vocabulary (one row, mxfp4), this takes 62.5; with one far value in x 140, with one in each of its
+// 90 groups 1170.
 template <bool INT4, bool PAIRED, int P, bool FAR>
 __device__ __forceinline__ void mv_tiles(const MatvecArgs& a, MvShared<P>& sh, uint8_t* dyn, MvRun& r) {
     using namespace moe::tc5;

@@ -146,7 +146,9 @@ moe_b200_status moe_b200_add_rmsnorm(const moe_b200_add_rmsnorm_args* args, moe_
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     // Chunks of 256 columns per warp.  Few rows want threads, many rows registers in flight; 1, 2 and 4 chunks, us (bf16,
     // fp32 residual, MX codes): 1 x 2880 2.5, 3.0, 5.1; 256 x 2880 3.6, 3.6, 6.0; 400 x 8192 12.4, 11.1, 14.1; 16384 x 1024 34.7,
-    // 35.8, 57.7; 16384 x 2880 97, 95, 146; 5000 x 8192 106, 83, 127.  A block has 32 warps at most.
+    // 35.8, 57.7; 16384 x 2880 97, 95, 146; 5000 x 8192 106, 83, 127.  A block has 32 warps at most, so rows of more than
+    // 16384 columns need four, and these do not fit the registers of 1024 threads: up to 800 bytes of a thread go to
+    // local memory.  1 x 32768 14.4; 1000 x 32768 114, 66 at the HBM rate.
     const int chunks = (H + 255) / 256;
     const int nv = chunks <= 32 ? (n_rows > 2 * sms && chunks > 4 ? 2 : 1) : chunks <= 64 ? 2 : 4;
     const int threads = 32 * ((chunks + nv - 1) / nv);
@@ -309,8 +311,8 @@ moe_b200_status moe_b200_w4_matvec(const moe_b200_w4_matvec_args* args, moe_b200
 
     // Pairs of x rows per pass over the weights.  Chosen matrices are shared by n_rows / n_mats rows on the average.
     // Two pairs halve what is read, but a step has twice the MMAs and the list half the items.  One and two, us:
-    // a matrix of its own per row (32 of 2880 x 2880) 30.3, 34.5; three or four rows per matrix 5.6, 6.9 (2048 x 2880),
-    // 8.4, 9.9 (5120), 10.1, 10.1 (8192), 28.9, 26.1 (40224), 14.9, 16.0 (4 x 2880), 24.0, 23.4 (8 x 2880).
+    // a matrix of its own per row (32 of 2880 x 2880) 29.6, 35.1; four rows per matrix 5.8, 7.3 (2048 x 2880),
+    // 8.2, 9.6 (5120), 9.7, 10.2 (8192), 28.7, 25.7 (40224), 14.6, 17.7 (4 x 2880), 25.5, 27.5 (8 x 2880).
     const int share = ids ? (n_rows + w->n_mats - 1) / w->n_mats : n_rows;
     const long long shared_items = (long long)(ids ? w->n_mats : 1) * ((share + 3) / 4) * a.n_tiles;
     int pairs = share <= 2 || shared_items < 5LL * sms ? 1 : 2;
@@ -318,11 +320,11 @@ moe_b200_status moe_b200_w4_matvec(const moe_b200_w4_matvec_args* args, moe_b200
     a.scale_slot = (MV_TILE * SG * sb + 15) / 16 * 16;
     a.scale_bulk = ((reinterpret_cast<uintptr_t>(w->scales) | (ids ? (unsigned long long)N * SG * sb : 0)) & 15) == 0;
     // The ring: rows in as few pieces as leave room for two stages in each of two blocks per SM, or for three in one.
-    // Us per 20000 rows, blocks per SM / steps of a piece / stages: 3584 columns 11.4 (2/28/2), 11.7 (2/28/3),
-    // 13.3 (1/28/4), 16.2 (2/24/3); 6144 20.5 (1/48/3), 20.9 (2/24/3), 25.4 (1/32/4); 8192 25.3 (1/64/2), 25.5 (2/32/2),
-    // 27.4 (1/32/4), 30.9 (2/16/4); 16384 44.7 (1/48/3), 45.0 (1/64/2), 53.0 (2/24/2).  Where x leaves two pairs only
-    // short pieces, two passes are faster: 4 rows, two pairs and one: 16384 columns 107 (1/16/3), 96; int4 176 (1/8/4),
-    // 105; 12288 int4 70 (1/24/3), 80.
+    // Us per 20000 rows, blocks per SM / steps of a piece / stages: 3584 columns 13.4 (2/28/2), 13.6 (2/28/3),
+    // 13.6 (1/28/4), 16.6 (2/24/3); 6144 18.9 (1/48/3), 19.8 (1/48/4), 20.9 (2/24/3), 25.2 (1/32/4); 8192 24.8 (1/64/2),
+    // 25.4 (2/32/2), 27.6 (1/32/4), 30.6 (2/16/4); 16384 44.3 (1/48/3), 44.2 (1/64/2), 53.4 (2/24/2).  Where x leaves two
+    // pairs only short pieces, two passes are faster: 4 rows, two pairs and one: 16384 columns 110 (1/16/3), 98; int4
+    // 179 (1/8/4), 118; 12288 int4 73 (1/24/3), 86.
     size_t smem = 0;
     int blocks = 0;
     for (;; pairs /= 2) {
