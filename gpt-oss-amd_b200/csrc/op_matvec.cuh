@@ -31,7 +31,7 @@
 //
 // Measured (201088 x 2880, mxfp4, one row: 308 MB, 48 us at the HBM rate).  Loads into registers, 8 rows x 64
 // bytes per instruction: 82 us with 32 warps per SM; a ring per warp filled by cp.async in the same
-// pattern: 72; a bulk copy per row: 81; one bulk copy per tile: 62.5.  Now 132 instructions per warp and step
+// pattern: 72; a bulk copy per row: 81; one bulk copy per tile: 62.  Now 132 instructions per warp and step
 // (56 of them decoding) at 2.2 per clock pace it: 60 clocks per step and SM against 44 at the HBM rate.  int4
 // decodes in 9 operations per 8 codes instead of 7: 81 us; a second pair of x rows adds 8 MMAs and
 // their x to a step: 86 us for three rows in mxfp4, 101 in int4.  Four pairs per pass were slower than two passes (230 us
@@ -313,11 +313,12 @@ __device__ __forceinline__ unsigned long long mv_far_groups(const MatvecArgs& a,
     return all;
 }
 
-// What is far in a row of x, in those groups, times rows n and n + 8 of a matrix; the four lanes of a quad have the
-// same n and share the 32 columns of a group.  From global memory.
+// What is far in a row of x, in those groups, times two rows of a matrix, the same for the four lanes of a quad, which
+// share the 32 columns of a group.  Codes and scales of the rows from their first group on.
 template <bool INT4>
-__device__ __forceinline__ float2 mv_far(const MatvecArgs& a, int mat, int n, long long xr, unsigned long long groups) {
-    const int lane = threadIdx.x & 31, t = lane & 3, G = a.K >> 5, SG = G >> a.group_shift;
+__device__ __forceinline__ float2 mv_far(const MatvecArgs& a, long long xr, unsigned long long groups, const uint8_t* codes0,
+                                         const uint8_t* codes1, const uint8_t* scales0, const uint8_t* scales1) {
+    const int lane = threadIdx.x & 31, t = lane & 3;
     const bool bf16 = a.x_dtype == MOE_B200_DTYPE_BF16;
     auto weight = [](uint32_t n) {
         if (INT4)
@@ -326,29 +327,35 @@ __device__ __forceinline__ float2 mv_far(const MatvecArgs& a, int mat, int n, lo
         const float v = m < 2 ? 0.5f * m : 0.25f * ((2 + (m & 1)) << (m >> 1));
         return n & 8 ? -v : v;
     };
-    auto scale = [&](size_t i) {
-        return INT4 ? half_to_float(static_cast<const uint16_t*>(a.scales)[i], MOE_B200_DTYPE_BF16)
-                    : e8m0_to_float(static_cast<const uint8_t*>(a.scales)[i]);
+    auto scale = [&](const uint8_t* row, int grp) {
+        return INT4 ? half_to_float(reinterpret_cast<const uint16_t*>(row)[grp >> a.group_shift], MOE_B200_DTYPE_BF16) : e8m0_to_float(row[grp]);
     };
     double lo = 0.0, hi = 0.0;
 #pragma unroll 1
     for (; groups; groups &= groups - 1) {
         const int at = __ffsll(groups) - 1, grp = ((int)(threadIdx.x >> 5) + (at >> 2) * MV_WARPS) * 4 + (at & 3);
+        const uint32_t w0 = *reinterpret_cast<const uint32_t*>(codes0 + grp * 16 + t * 4);
+        const uint32_t w1 = *reinterpret_cast<const uint32_t*>(codes1 + grp * 16 + t * 4);
         const long long col = xr * a.x_stride + grp * 32 + t * 8;
-        const size_t row0 = (size_t)mat * a.N + min(n, a.N - 1), row1 = (size_t)mat * a.N + min(n + 8, a.N - 1);
-        uint32_t w0 = *reinterpret_cast<const uint32_t*>(a.codes + (row0 * G + grp) * 16 + t * 4);
-        uint32_t w1 = *reinterpret_cast<const uint32_t*>(a.codes + (row1 * G + grp) * 16 + t * 4);
-        const float s0 = scale(row0 * SG + (grp >> a.group_shift)), s1 = scale(row1 * SG + (grp >> a.group_shift));
-        uint32_t span = 0;
+        // columns that are far in any of the four lanes, and what they are of
+        uint32_t todo = 0xFF, span = 0;
         if (bf16) {
             const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + col);
             const uint32_t h[4] = {v.x, v.y, v.z, v.w};
             span = mv_span(h, lane);
+            if (!mv_far_group(span)) {
+                todo = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    todo |= (mv_far_value(h[e], span) ? 1u : 0u) << (2 * e) | (mv_far_value(h[e] >> 16, span) ? 2u : 0u) << (2 * e);
+                todo = __reduce_or_sync(0xffffffffu, todo);
+            }
         }
         const bool whole = mv_far_group(span);
         double d0 = 0.0, d1 = 0.0;
 #pragma unroll 1
-        for (int i = 0; i < 8; i++) {
+        for (; todo; todo &= todo - 1) {
+            const int i = __ffs(todo) - 1;
             float x;
             if (bf16) {
                 const uint32_t bits = static_cast<const uint16_t*>(a.x)[col + i];
@@ -358,12 +365,11 @@ __device__ __forceinline__ float2 mv_far(const MatvecArgs& a, int mat, int n, lo
                 v.__x = static_cast<const uint8_t*>(a.x)[col + i];
                 x = (float)v;
             }
-            d0 += (double)weight(w0 & 15) * (double)x;
-            d1 += (double)weight(w1 & 15) * (double)x;
-            w0 >>= 4, w1 >>= 4;
+            d0 += (double)weight(w0 >> (4 * i) & 15) * (double)x;
+            d1 += (double)weight(w1 >> (4 * i) & 15) * (double)x;
         }
         const double sx = bf16 ? 1.0 : (double)mv_x_scale(a, xr, grp);
-        d0 *= sx * (double)s0, d1 *= sx * (double)s1;
+        d0 *= sx * (double)scale(scales0, grp), d1 *= sx * (double)scale(scales1, grp);
         d0 += __shfl_xor_sync(0xffffffffu, d0, 1), d1 += __shfl_xor_sync(0xffffffffu, d1, 1);
         lo += d0 + __shfl_xor_sync(0xffffffffu, d0, 2), hi += d1 + __shfl_xor_sync(0xffffffffu, d1, 2);
     }
@@ -389,8 +395,8 @@ struct MvRun {
 };
 
 // The sums of the tiles of a pass.  FAR: something of its x is far.  Two instances: one with a test at the end of a tile
-// took 66 us for the vocabulary (one row, mxfp4), this takes 62.5; with one far value in x 140, with one in each of its
-// 90 groups 1170.
+// took 66 us for the vocabulary (one row, mxfp4), this takes 62; with one far value in x 102, with one in each of its
+// 90 groups 560.
 template <bool INT4, bool PAIRED, int P, bool FAR>
 __device__ __forceinline__ void mv_tiles(const MatvecArgs& a, MvShared<P>& sh, uint8_t* dyn, MvRun& r) {
     using namespace moe::tc5;
@@ -494,7 +500,14 @@ __device__ __forceinline__ void mv_tiles(const MatvecArgs& a, MvShared<P>& sh, u
                     if constexpr (FAR)
 #pragma unroll 1
                         for (int c = 2 * p; c < min(2 * p + 2, r.cnt); c++) {
-                            const float2 f = mv_far<INT4>(a, a.ids ? sh.ids[sh.lead[r.li]] : 0, r.tile * MV_TILE + gr, sh.rows[c] / a.rows_per_x, far[c]);
+                            if (!far[c])
+                                continue;
+                            // the stage has whole rows, or their last pieces
+                            const int n = r.tile * MV_TILE + gr;
+                            const size_t row = (size_t)(a.ids ? sh.ids[sh.lead[r.li]] : 0) * a.N;
+                            const uint8_t* codes0 = c0 == 0 ? dyn + 128 + r.stage * stage_bytes + gr * a.pitch : a.codes + (row + min(n, a.N - 1)) * G * 16;
+                            const uint8_t* codes1 = c0 == 0 ? codes0 + 8 * a.pitch : a.codes + (row + min(n + 8, a.N - 1)) * G * 16;
+                            const float2 f = mv_far<INT4>(a, sh.rows[c] / a.rows_per_x, far[c], codes0, codes1, dyn + scales_row, dyn + scales_row + 8 * SG * SB);
                             if (c == 2 * p + (t >> 1)) {
                                 lo += f.x;
                                 hi += f.y;

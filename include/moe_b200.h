@@ -518,8 +518,8 @@ typedef struct {
  * Products are exact and summed in fp32, a row's in an order that depends on cols
  * alone; one rounding at the end.  That holds for x and scales of any size: what the
  * fast path cannot hold (bf16 values more than 2^31 below the largest of their 32
- * columns, x scales beyond 2^-100..2^103) is added in a slower one, 2.2 times the time
- * for one such value in a row.  Many rows of one matrix read its codes once per 2 or 4
+ * columns, x scales beyond 2^-100..2^103) is added in a slower one: up to twice the
+ * time for one such value in a row.  Many rows of one matrix read its codes once per 2 or 4
  * of them too: 5120 x 2880 in MXFP4 takes 5.8 us for one row, 11 for 8, 41 for 64, 136
  * for 256.  Row addresses of x must be 16-byte aligned (8
  * bytes for e4m3).  The kernel's waits for its own copies are bounded (2 s): rows

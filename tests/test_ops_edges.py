@@ -179,6 +179,44 @@ def test_matvec_x_scales_of_zero_infinity_and_nan():
     assert (y[0] == 32).all() and (y[1] == math.inf).all() and y[2].isnan().all() and (y[3] == -48).all()
 
 
+@pytest.mark.parametrize("fmt,K", [("mxfp4", 544), ("int4", 544), ("mxfp4", 11264)])
+@pytest.mark.parametrize("kind", ["values", "group", "e4m3"])
+def test_matvec_far_rows_through_chosen_matrices(fmt, K, kind):
+    """Rows that need the slower path, shared by several matrices, with a bias and the SwiGLU, beside rows that do not
+    and rows without a matrix."""
+    g = _gen(K)
+    n, N, rows, rpx = 5, 70, 6, 3
+    codes, scales = _weights(g, (n,), N, K, fmt, 32)
+    bias = 0.1 * _randn(g, n, N)
+    ids = torch.tensor([0, 4, 4, -1, 4, 2, 4, 4, 0, 9, 3, 3, 4, 0, 1, 2, 2, 2], dtype=torch.int32, device="cuda")
+    wide = _randn(g, rows, K + 8).to(BF16)
+    x, xs, x64 = wide[:, :K], None, None
+    if kind == "values":
+        x[1, 5::96] = 2.0**-70
+        x[4, K - 1] = -(2.0**-40)
+    elif kind == "group":
+        x[1, 32:96] *= 2.0**-110
+        x[4, K - 32:] *= 2.0**120
+        scales[:, :, K // 32 - 1:] = 10 if fmt == "mxfp4" else 2.0**-115
+    else:
+        x = x.float().to(torch.float8_e4m3fn)
+        e = torch.zeros(rows, K // 32, device="cuda")
+        e[1, 1:3] = -112
+        e[4, -1] = 110
+        xs = (e + 127).to(torch.uint8)
+        scales[:, :, K // 32 - 1:] = 10 if fmt == "mxfp4" else 2.0**-115
+        x64 = x.double() * torch.exp2(e.double()).repeat_interleave(32, 1)
+    x64 = x.double() if x64 is None else x64
+    for act in (None, (1.702, 7.0)):
+        y = pkg.w4_matvec(x, codes, scales, bias, x_scales=xs, ids=ids, rows_per_x=rpx, swiglu=act, dtype=F32)
+        _check_matvec(y, x64, codes, scales, bias, 32, ids, rpx, act)
+        assert (y[[3, 9]] == 0).all()
+        for m in (1, 4, 13):
+            one = pkg.w4_matvec(x[m // rpx:m // rpx + 1], codes, scales, bias, x_scales=None if xs is None else xs[m // rpx:m // rpx + 1],
+                                ids=ids[m:m + 1], swiglu=act, dtype=F32)
+            assert torch.equal(y[m:m + 1], one)
+
+
 # -- calls beside other work ---------------------------------------------------------------
 
 
