@@ -31,10 +31,10 @@
 //
 // Measured (201088 x 2880, mxfp4, one row: 308 MB, 48 us at the HBM rate).  Loads into registers, 8 rows x 64
 // bytes per instruction: 82 us with 32 warps per SM; a ring per warp filled by cp.async in the same
-// pattern: 72; a bulk copy per row: 81; one bulk copy per tile: 62.  Now 132 instructions per warp and step
-// (56 of them decoding) at 2.2 per clock pace it: 60 clocks per step and SM against 44 at the HBM rate.  int4
+// pattern: 72; a bulk copy per row: 81; one bulk copy per tile: 62.  Now 134 instructions per warp and step
+// (56 of them decoding) at 2.3 per clock pace it: 59 clocks per step and SM against 44 at the HBM rate.  int4
 // decodes in 9 operations per 8 codes instead of 7: 81 us; a second pair of x rows adds 8 MMAs and
-// their x to a step: 86 us for three rows in mxfp4, 101 in int4.  Four pairs per pass were slower than two passes (230 us
+// their x to a step: 85 us for three rows in mxfp4, 101 in int4.  Four pairs per pass were slower than two passes (230 us
 // against 164).
 #pragma once
 #include "common.cuh"

@@ -395,7 +395,8 @@ moe_b200_status moe_b200_route_noalloc(const void* t, int t_dtype, int n_tokens,
  * allocation, nothing kept between calls: calls may overlap on any streams and
  * host threads and may be captured into graphs.  Device pointers and a stream of
  * the current device.  Strides are in elements between two rows.  Nothing outside
- * the stated rows and columns is written.  The kernels wait for all work in front of
+ * the stated rows and columns is written.  Outputs overlap neither inputs nor each
+ * other, but where it is said that they may.  The kernels wait for all work in front of
  * them; a kernel that the caller launches behind one as its programmatic dependent has
  * to wait too (griddepcontrol.wait) before it touches their tensors. */
 
@@ -520,7 +521,7 @@ typedef struct {
  * fast path cannot hold (bf16 values more than 2^31 below the largest of their 32
  * columns, x scales beyond 2^-100..2^103) is added in a slower one: up to twice the
  * time for one such value in a row.  Many rows of one matrix read its codes once per 2 or 4
- * of them too: 5120 x 2880 in MXFP4 takes 5.8 us for one row, 11 for 8, 41 for 64, 136
+ * of them too: 5120 x 2880 in MXFP4 takes 5.9 us for one row, 11 for 8, 41 for 64, 136
  * for 256.  Row addresses of x must be 16-byte aligned (8
  * bytes for e4m3).  The kernel's waits for its own copies are bounded (2 s): rows
  * behind one that ran out become NaN. */
